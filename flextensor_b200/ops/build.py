@@ -26,6 +26,7 @@ SOURCES = [
     "tp_sm100.cu",
     "moe_sm100.cu",
     "decode_sm100.cu",
+    "cache_q8_sm100.cu",
 ]
 
 CUDA_FLAGS = [
@@ -35,6 +36,15 @@ CUDA_FLAGS = [
     "-U__CUDA_NO_HALF_OPERATORS__", "-U__CUDA_NO_BFLOAT16_CONVERSIONS__",
 ]
 CXX_FLAGS = ["-O3", "-std=c++17"]
+
+
+def _shared_cxx_runtime() -> list[str]:
+    """The C++ runtime library that torch has loaded, as a link input. A compiler that would link
+    its own static copy instead leaves two runtimes in the process, and the first stream that a
+    binding uses to format an error message with a number in it crashes."""
+    with open("/proc/self/maps") as f:
+        paths = {line.split()[-1] for line in f if "/libstdc++.so" in line}
+    return sorted(paths)[:1]
 
 
 def build(verbose: bool = False):
@@ -51,6 +61,7 @@ def build(verbose: bool = False):
         extra_cuda_cflags=CUDA_FLAGS + extra,
         extra_cflags=CXX_FLAGS,
         extra_include_paths=[str(CSRC)],
+        extra_ldflags=_shared_cxx_runtime(),
         with_cuda=True,
         verbose=verbose,
     )
