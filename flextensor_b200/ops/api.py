@@ -141,6 +141,56 @@ def decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out
 
 
+def kv_append_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                 v_scale: torch.Tensor, pos: int | torch.Tensor, *, block: int = 64,
+                 n_new: torch.Tensor | None = None) -> None:
+    """Write new tokens into a key/value cache held in 8 bits, in place.
+
+    ``k`` / ``v`` bf16 ``[B, S, Hk, 128]`` go to positions ``[pos, pos + S)`` of the codes
+    ``k_cache`` / ``v_cache [B, L, Hk, 128]`` (``torch.int8`` or ``torch.float8_e4m3fn``) with fp32
+    scales ``[B, ceil(L / block), Hk]``, one per ``block`` tokens (16 to 256, a power of two) and
+    head: the value of a code is ``code * scale``. ``pos``: an int (every sequence) or int32 CUDA
+    ``[B]``. ``n_new`` (int32 CUDA ``[B]``): tokens to take of each sequence's S; the rest are
+    padding, not read.
+
+    A block's scale is the smallest power of two with ``max|x| <= 127 * scale`` (448 for e4m3; 0
+    for a block of zeros, never below 2**-120). A block whose first position is written starts
+    afresh; one that holds earlier tokens of the sequence keeps the larger of its scale and the new
+    tokens', and its codes are rounded again when that grows. A NaN or infinity makes its block's
+    scale NaN, so that attention over it answers NaN. Codes outside the written tokens and their
+    blocks' earlier ones stay as they were. A sequence whose device-side ``pos`` / ``n_new`` do not
+    fit the cache is left alone and recorded in ``native.device_error``."""
+    if isinstance(pos, torch.Tensor):
+        native.lib().kv_append_q8(k, v, k_cache, v_cache, k_scale, v_scale, pos, 0, n_new, block)
+    else:
+        native.lib().kv_append_q8(k, v, k_cache, v_cache, k_scale, v_scale, None, pos, n_new, block)
+    _count()
+
+
+def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                        v_scale: torch.Tensor, kv_len: int | torch.Tensor, *, block: int = 64,
+                        max_len: int | None = None, scale: float | None = None,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`decode_attention` over a cache written by :func:`kv_append_q8` (or any codes with
+    scales that are not negative; e4m3 codes must be finite).
+
+    ``q [B, Hq, 128]``, or ``[B, Sq, Hq, 128]`` for the last Sq tokens of each sequence, whose keys
+    are in the cache already: query i sees keys ``[0, kv_len - Sq + 1 + i)``; one that sees none
+    gets zeros. ``kv_len``: an int or an int32 CUDA tensor ``[B]`` (then ``max_len``, default L,
+    bounds it: longer ones are cut)."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1])
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if isinstance(kv_len, torch.Tensor):
+        ml = k_cache.shape[1] if max_len is None else max_len
+        n = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, kv_len, 0, ml, block, scale)
+    else:
+        n = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, None, kv_len, kv_len, block, scale)
+    _count(n)
+    return out
+
+
 def attention_cp(q: torch.Tensor, kv_local: torch.Tensor, *, peer_kv: list[int], flags_ptr: int, flag_stride: int,
                  peer_acks: list[int], rank: int, shard_rows: int, epoch: int, counters: torch.Tensor,
                  scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:

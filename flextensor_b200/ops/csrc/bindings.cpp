@@ -2,6 +2,7 @@
 //
 // Every op validates device, dtype, shape and stride before launching and
 // launches on the caller's current CUDA stream; a failed launch raises.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -9,6 +10,7 @@
 #include <cstdlib>
 
 #include "ft_attn.h"
+#include "ft_cache.h"
 #include "ft_ops.h"
 #include "ft_ops_norm.h"
 #include "ft_runtime.h"
@@ -269,6 +271,165 @@ void decode_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, Tenso
   }
   const cudaError_t e = ft::decode_attention(p, at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(e == cudaSuccess, "decode_attention: ", cudaGetErrorString(e));
+}
+
+// ---- key/value cache in 8 bits. Shapes, types and strides are checked before the device, so a
+// refused call says why on any machine.
+constexpr int64_t kHead = 128;
+
+bool on_16_bytes(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+
+void check_cache(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, int64_t block, const char* op) {
+  TORCH_CHECK(kc.dim() == 4 && kc.size(3) == kHead && vc.sizes() == kc.sizes(), op,
+              ": k_cache and v_cache must be [B, L, Hk, 128] of one shape, got ", kc.sizes(), " and ", vc.sizes());
+  TORCH_CHECK((kc.scalar_type() == at::kChar || kc.scalar_type() == at::kFloat8_e4m3fn) &&
+                  vc.scalar_type() == kc.scalar_type(),
+              op, ": the caches must both be int8 or both float8_e4m3fn");
+  TORCH_CHECK(block == 16 || block == 32 || block == 64 || block == 128 || block == 256, op,
+              ": block must be 16, 32, 64, 128 or 256 tokens, got ", block);
+  TORCH_CHECK(kc.size(1) < (1LL << 30), op, ": the cache is too long");
+  const std::vector<int64_t> want = {kc.size(0), (kc.size(1) + block - 1) / block, kc.size(2)};
+  TORCH_CHECK(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat && ks.sizes() == at::IntArrayRef(want) &&
+                  vs.sizes() == at::IntArrayRef(want),
+              op, ": scales must be fp32 [B, ceil(L / block), Hk] = ", at::IntArrayRef(want), ", got ", ks.sizes(), " and ",
+              vs.sizes());
+  for (const Tensor* t : {&kc, &vc}) {
+    TORCH_CHECK(t->stride(3) == 1 && t->stride(0) % 16 == 0 && t->stride(1) % 16 == 0 && t->stride(2) % 16 == 0 &&
+                    on_16_bytes(*t),
+                op, ": cache rows must be contiguous and start on 16-byte boundaries");
+  }
+}
+
+ft::CacheSide cache_side(const Tensor& c, const Tensor& s) {
+  ft::CacheSide x;
+  x.codes = reinterpret_cast<uint8_t*>(c.data_ptr());
+  x.c_b = c.stride(0);
+  x.c_tok = c.stride(1);
+  x.c_h = c.stride(2);
+  x.scale = s.data_ptr<float>();
+  x.s_b = s.stride(0);
+  x.s_blk = s.stride(1);
+  x.s_h = s.stride(2);
+  return x;
+}
+
+// rows of 128 bf16 values that 16-byte loads can take
+void check_rows(const Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16, op, ": ", name, " must be bfloat16");
+  TORCH_CHECK(t.dim() == 4 && t.size(3) == kHead, op, ": ", name, " must be [B, S, H, 128], got ", t.sizes());
+  TORCH_CHECK(t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 && on_16_bytes(t),
+              op, ": rows of ", name, " must be contiguous and start on 16-byte boundaries");
+}
+
+void check_lengths(const c10::optional<Tensor>& t, int64_t B, const char* op, const char* name) {
+  if (!t || !t->defined()) return;
+  TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B && t->is_contiguous(), op, ": ", name,
+              " must be a contiguous int32 tensor with one number per sequence");
+}
+
+void check_same_cuda(const Tensor& first, std::initializer_list<const Tensor*> rest, const char* op) {
+  TORCH_CHECK(first.is_cuda(), op, ": tensors must be on a CUDA device");
+  for (const Tensor* t : rest)
+    TORCH_CHECK(!t->defined() || t->device() == first.device(), op, ": all tensors must be on one device");
+}
+
+void kv_append_q8(const Tensor& k, const Tensor& v, Tensor& kc, Tensor& vc, Tensor& ks, Tensor& vs,
+                  const c10::optional<Tensor>& pos, int64_t pos_all, const c10::optional<Tensor>& n_new, int64_t block) {
+  const char* op = "kv_append_q8";
+  check_cache(kc, vc, ks, vs, block, op);
+  check_rows(k, op, "k");
+  check_rows(v, op, "v");
+  const int64_t B = kc.size(0), L = kc.size(1), Hk = kc.size(2), S = k.size(1);
+  TORCH_CHECK(k.size(0) == B && k.size(2) == Hk && v.sizes() == k.sizes(), op, ": k and v must be [B, S, Hk, 128] with B = ",
+              B, " and Hk = ", Hk, ", got ", k.sizes(), " and ", v.sizes());
+  check_lengths(pos, B, op, "pos");
+  check_lengths(n_new, B, op, "n_new");
+  const bool each = pos && pos->defined();
+  TORCH_CHECK(S <= L, op, ": ", S, " new tokens do not fit a cache of ", L);
+  if (!each)
+    TORCH_CHECK(pos_all >= 0 && (n_new && n_new->defined() ? pos_all <= L : pos_all + S <= L), op, ": tokens [", pos_all,
+                ", ", pos_all + S, ") do not fit a cache of ", L);
+  for (const Tensor* t : {&kc, &vc, &ks, &vs})
+    TORCH_CHECK(at::has_internal_overlap(*t) != at::MemOverlap::Yes, op, ": the cache must not overlap itself");
+  at::assert_no_overlap(kc, vc);
+  at::assert_no_overlap(ks, vs);
+  check_same_cuda(kc, {&vc, &ks, &vs, &k, &v}, op);
+  if (each) check_same_cuda(kc, {&*pos}, op);
+  if (n_new && n_new->defined()) check_same_cuda(kc, {&*n_new}, op);
+  c10::cuda::CUDAGuard g(kc.device());
+  ft::CacheAppendProblem p;
+  p.B = (int)B;
+  p.S = (int)S;
+  p.Hk = (int)Hk;
+  p.L = (int)L;
+  p.block = (int)block;
+  p.format = kc.scalar_type() == at::kChar ? ft::CACHE_INT8 : ft::CACHE_E4M3;
+  const Tensor* x[2] = {&k, &v};
+  for (int i = 0; i < 2; i++) {
+    p.x[i] = reinterpret_cast<const __nv_bfloat16*>(x[i]->data_ptr());
+    p.x_b[i] = x[i]->stride(0);
+    p.x_tok[i] = x[i]->stride(1);
+    p.x_h[i] = x[i]->stride(2);
+  }
+  p.side[0] = cache_side(kc, ks);
+  p.side[1] = cache_side(vc, vs);
+  p.pos = each ? pos->data_ptr<int>() : nullptr;
+  p.pos_all = (int)pos_all;
+  p.n_new = n_new && n_new->defined() ? n_new->data_ptr<int>() : nullptr;
+  check_ok(ft::cache_append(p, at::cuda::getCurrentCUDAStream()), op);
+}
+
+// returns the number of kernels launched
+int64_t decode_attention_q8(const Tensor& q_in, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
+                            Tensor& o_in, const c10::optional<Tensor>& kv_len, int64_t len_all, int64_t max_len,
+                            int64_t block, double scale) {
+  const char* op = "decode_attention_q8";
+  check_cache(kc, vc, ks, vs, block, op);
+  const Tensor q = q_in.dim() == 3 ? q_in.unsqueeze(1) : q_in;
+  const Tensor o = o_in.dim() == 3 ? o_in.unsqueeze(1) : o_in;
+  check_rows(q, op, "q");
+  check_rows(o, op, "out");
+  const int64_t B = kc.size(0), L = kc.size(1), Hk = kc.size(2), Sq = q.size(1), Hq = q.size(2);
+  TORCH_CHECK(q.size(0) == B, op, ": q has ", q.size(0), " sequences, the cache ", B);
+  TORCH_CHECK(o.sizes() == q.sizes(), op, ": out must have the shape of q");
+  TORCH_CHECK(Hk > 0 && Hq % Hk == 0, op, ": query heads must be a multiple of kv heads, got ", Hq, " and ", Hk);
+  check_lengths(kv_len, B, op, "kv_len");
+  TORCH_CHECK(max_len >= 0 && max_len <= L && len_all >= 0 && len_all <= L, op, ": lengths must lie in [0, ", L, "]");
+  TORCH_CHECK(at::has_internal_overlap(o) != at::MemOverlap::Yes, op, ": out must not overlap itself");
+  check_same_cuda(kc, {&vc, &ks, &vs, &q, &o}, op);
+  const bool each = kv_len && kv_len->defined();
+  if (each) check_same_cuda(kc, {&*kv_len}, op);
+  c10::cuda::CUDAGuard g(kc.device());
+  ft::CacheDecodeProblem p;
+  p.B = (int)B;
+  p.Sq = (int)Sq;
+  p.Hq = (int)Hq;
+  p.Hk = (int)Hk;
+  p.L = (int)L;
+  p.block = (int)block;
+  p.format = kc.scalar_type() == at::kChar ? ft::CACHE_INT8 : ft::CACHE_E4M3;
+  p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
+  p.q_b = q.stride(0);
+  p.q_tok = q.stride(1);
+  p.q_h = q.stride(2);
+  p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
+  p.o_b = o.stride(0);
+  p.o_tok = o.stride(1);
+  p.o_h = o.stride(2);
+  p.side[0] = cache_side(kc, ks);
+  p.side[1] = cache_side(vc, vs);
+  p.kv_len = each ? kv_len->data_ptr<int>() : nullptr;
+  p.len_all = (int)len_all;
+  p.max_len = (int)(each ? max_len : len_all);
+  p.scale = (float)scale;
+  p.num_sms = num_sms_for(kc.get_device());
+  Tensor scratch;
+  if (const size_t n = ft::cache_decode_scratch_floats(p)) {
+    scratch = at::empty({(int64_t)n}, ks.options());
+    p.scratch = scratch.data_ptr<float>();
+  }
+  check_ok(ft::cache_decode(p, at::cuda::getCurrentCUDAStream()), op);
+  return ft::cache_decode_launches(p);
 }
 
 void attention_cp(const Tensor& q, const Tensor& kv_local, Tensor& o, double scale, std::vector<uint64_t> peer_kv,
@@ -631,7 +792,8 @@ int device_error(bool reset) {
   int t = ft::tp_device_error(reset);
   int m = ft::moe_device_error(reset);
   int d = ft::decode_device_error(reset);
-  return e ? e : (n ? n : (a ? a : (p ? p : (t ? t : (m ? m : d)))));
+  int c = ft::cache_device_error(reset);
+  return e ? e : (n ? n : (a ? a : (p ? p : (t ? t : (m ? m : (d ? d : c))))));
 }
 
 struct PyEngine {
@@ -737,6 +899,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention", &decode_attention, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("out"),
         py::arg("seqlens"), py::arg("kv_len"), py::arg("max_len"), py::arg("scale"), py::arg("n_split") = 0);
   m.def("decode_splits", [](int B, int Hk, int max_len, int num_sms) { return ft::decode_splits(B, Hk, max_len, num_sms); });
+  m.def("kv_append_q8", &kv_append_q8, py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("k_scale"), py::arg("v_scale"), py::arg("pos"), py::arg("pos_all"), py::arg("n_new"), py::arg("block"));
+  m.def("decode_attention_q8", &decode_attention_q8, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("k_scale"), py::arg("v_scale"), py::arg("out"), py::arg("kv_len"), py::arg("len_all"),
+        py::arg("max_len"), py::arg("block"), py::arg("scale"));
   m.def("p2p_publish_raw", &p2p_publish_raw);
   m.def("tp_ag_gemm", &tp_ag_gemm, py::arg("a_full"), py::arg("w"), py::arg("out"), py::arg("bias"), py::arg("epi"),
         py::arg("peer_a"), py::arg("flags"), py::arg("flag_stride"), py::arg("peer_acks"), py::arg("rank"),

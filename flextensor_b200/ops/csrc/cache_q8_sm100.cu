@@ -1,0 +1,632 @@
+// Key/value cache in 8 bits with one scale per block of tokens and head: writing tokens into it
+// and decode attention over it, head_dim 128, for sm_100a.
+//
+// Writing. A block's scale is the smallest power of two s with max|x| <= qmax * s (qmax 127 for
+// int8, 448 for e4m3), so x / s is exact and a code depends on the value alone; a block that
+// already holds tokens keeps the larger of its old scale and the new tokens', and its old codes
+// are rounded again when the scale grew. The largest magnitude is found on the bf16 bit patterns
+// (sign cleared, as 16-bit integers): NaN and infinity compare above every finite value, and a
+// block that received one gets the scale NaN, which reaches every output that reads the block.
+//
+// Decode attention. Per cached token and KV head 256 code bytes are read once and each takes part
+// in 2 * G * Sq multiply-adds, so the kernel is bound by HBM. The codes go to f16 in registers
+// (exact for both formats) and the products run as warp-level m16n8k16 MMAs with the *keys* on the
+// 16-row side and the query rows (heads of one KV group x query tokens) on the 8-column side:
+//   S^T[key, row] = K q^T,   O^T[dim, row] += V^T P^T.
+// Eight rows are one column tile, so a group of 8 heads wastes no MMA work. Which physical
+// dimension or key a fragment slot stands for is free as long as both operands agree, so every
+// lane takes its fragments from 16-byte pieces of the cache rows as they lie in memory:
+//   K: lane (g, c) holds rows g and g + 8 of a 16-key tile, dims 32c .. 32c+31;
+//   V: lane (g, c) holds rows 2c, 2c+1, 2c+8, 2c+9, dims 16g .. 16g+15; two rows' bytes are
+//      interleaved with PRMT into the (key, key+1) pairs the MMA wants.
+// P goes from the accumulator layout to the B operand with one 8x8 transpose per 8 keys.
+//
+// Scales: a score is (q . codes) * ks, and the weight of a value's codes is p * vs. The running
+// reference m is the maximum of score + log2(vs), so p * vs <= 1 whatever the scales are and f16
+// holds it to 2^-11 of the largest weight; the sum l takes p itself in fp32. q is scaled by a power
+// of two per row into f16 (exact but for elements below 2^-24 of the row's largest).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include "ft_cache.h"
+#include "sm100_common.cuh"
+
+namespace ft {
+
+FT_DEFINE_ERROR_READER(cache_device_error)
+
+namespace {
+
+constexpr int HD = 128;  // head dim
+
+// ------------------------------------------------------------------------------------ writing
+struct AppendArgs {
+  int B, S, Hk, L, n_rel;
+  const __nv_bfloat16* x[2];
+  long long x_b[2], x_tok[2], x_h[2];
+  CacheSide side[2];
+  const int* pos;
+  int pos_all;
+  const int* n_new;
+};
+
+// smallest power of two s with a <= qmax * s, for a bf16 magnitude given by its bits
+template <int FMT>
+__device__ __forceinline__ float pow2_scale(uint32_t bits) {
+  if (bits >= 0x7f80u) return __int_as_float(0x7fc00000);
+  if (bits == 0u) return 0.f;
+  // a = (1/2 + man/256) 2^e; qmax = 254/256 * 2^7 (int8), 224/256 * 2^9 (e4m3)
+  const int man = bits & 0x7f, e = (int)(bits >> 7) - 126;
+  const int k = FMT == CACHE_INT8 ? e - 7 + (man > 126) : e - 9 + (man > 96);
+  return __int_as_float((max(k, -120) + 127) << 23);
+}
+
+template <int FMT>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+  if (FMT == CACHE_INT8) {
+    const int ia = min(127, max(-127, __float2int_rn(a))), ib = min(127, max(-127, __float2int_rn(b)));
+    const int ic = min(127, max(-127, __float2int_rn(c))), id = min(127, max(-127, __float2int_rn(d)));
+    return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
+  }
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+// four codes of a word rounded again under a scale grown by 1 / ratio
+template <int FMT>
+__device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
+  float f[4];
+  if (FMT == CACHE_INT8) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = (float)(int8_t)(w >> (8 * i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)(w >> (8 * i)), __NV_E4M3)));
+  }
+  return encode4<FMT>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
+}
+
+// One CTA per (sequence, block of tokens, KV head, keys or values); the block's new tokens are
+// held in registers between the maximum and the rounding, so they are read once.
+template <int BLOCK, int FMT>
+__global__ void __launch_bounds__(BLOCK <= 64 ? 128 : 256) cache_append_kernel(AppendArgs a) {
+  constexpr int THREADS = BLOCK <= 64 ? 128 : 256;
+  constexpr int ROWS = THREADS / 16;  // token rows per pass: 16 lanes hold a row's 128 values
+  constexpr int ITERS = BLOCK / ROWS;
+  __shared__ uint32_t warp_max[THREADS / 32];
+  long long id = blockIdx.x;
+  const int h = (int)(id % a.Hk);
+  id /= a.Hk;
+  const int rel = (int)(id % a.n_rel);
+  id /= a.n_rel;
+  const int kv = (int)(id & 1), b = (int)(id >> 1);
+  const int p = a.pos ? a.pos[b] : a.pos_all, n = a.n_new ? a.n_new[b] : a.S;
+  if (p < 0 || n < 0 || n > a.S || p > a.L - n) {  // nothing of such a sequence is written
+    if (threadIdx.x == 0) record_error(kErrBadArgs);
+    return;
+  }
+  const int j = p / BLOCK + rel;
+  const int t0 = max(p, j * BLOCK), t1 = min(p + n, (j + 1) * BLOCK);
+  if (t0 >= t1) return;
+  const CacheSide& sd = a.side[kv];
+  float* const sp = sd.scale + b * sd.s_b + j * sd.s_blk + h * sd.s_h;
+  const bool history = t0 > j * BLOCK;
+  const float s_old = history ? *sp : 0.f;
+  const int row0 = threadIdx.x / 16, col = (threadIdx.x % 16) * 8;
+  const __nv_bfloat16* const x = a.x[kv] + b * a.x_b[kv] + h * a.x_h[kv] + col;
+  uint4 v[ITERS];
+  uint32_t m2 = 0;
+#pragma unroll
+  for (int i = 0; i < ITERS; i++) {
+    const int t = j * BLOCK + i * ROWS + row0;
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (t >= t0 && t < t1) v[i] = __ldg(reinterpret_cast<const uint4*>(x + (long long)(t - p) * a.x_tok[kv]));
+  }
+#pragma unroll
+  for (int i = 0; i < ITERS; i++) {
+    m2 = __vmaxu2(m2, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
+                               __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
+  }
+  uint32_t m = __reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16));
+  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
+  __syncthreads();  // also: every thread has read the old scale
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; w++) m = max(m, warp_max[w]);
+  const float s_new = pow2_scale<FMT>(m);
+  const float s = s_old != s_old ? s_old : (s_new != s_new ? s_new : fmaxf(s_old, s_new));
+  const bool bad = s != s;
+  const float inv = bad ? 0.f : (s > 0.f ? 1.f / s : 0.f);
+  uint8_t* const out = sd.codes + b * sd.c_b + h * sd.c_h + col;
+  if (history && s != s_old) {
+    const float ratio = bad ? 0.f : s_old * inv;
+    for (int t = j * BLOCK + row0; t < t0; t += ROWS) {
+      uint2* const w = reinterpret_cast<uint2*>(out + (long long)t * sd.c_tok);
+      const uint2 o = *w;
+      *w = bad ? make_uint2(0, 0) : make_uint2(recode4<FMT>(o.x, ratio), recode4<FMT>(o.y, ratio));
+    }
+  }
+  if (threadIdx.x == 0) *sp = s;
+#pragma unroll
+  for (int i = 0; i < ITERS; i++) {
+    const int t = j * BLOCK + i * ROWS + row0;
+    if (t < t0 || t >= t1) continue;
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      f[2 * e] = __uint_as_float(w[e] << 16) * inv;
+      f[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u) * inv;
+    }
+    uint2 o = make_uint2(encode4<FMT>(f[0], f[1], f[2], f[3]), encode4<FMT>(f[4], f[5], f[6], f[7]));
+    if (bad) o = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(out + (long long)t * sd.c_tok) = o;
+  }
+}
+
+template <int BLOCK>
+cudaError_t launch_append(const AppendArgs& a, int format, cudaStream_t stream) {
+  const long long grid = (long long)a.B * 2 * a.n_rel * a.Hk;
+  if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const int threads = BLOCK <= 64 ? 128 : 256;
+  if (format == CACHE_INT8) cache_append_kernel<BLOCK, CACHE_INT8><<<(unsigned)grid, threads, 0, stream>>>(a);
+  else cache_append_kernel<BLOCK, CACHE_E4M3><<<(unsigned)grid, threads, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+// ------------------------------------------------------------------------------------ attention
+constexpr int KT = 32;   // keys of a warp's tile
+constexpr int NWARP = 4;
+
+struct DecArgs {
+  int B, Sq, Hq, Hk, L, G, R, n_group;  // R = Sq * G query rows of a KV head; n_group column groups of 8 * NT rows
+  int block_shift;
+  const __nv_bfloat16* q;
+  long long q_b, q_tok, q_h;
+  __nv_bfloat16* o;
+  long long o_b, o_tok, o_h;
+  CacheSide k, v;
+  const int* kv_len;
+  int len_all, max_len;
+  float scale_log2;  // softmax scale * log2(e)
+  int n_split;
+  float* part_o;   // [n_split, B, Hk, R, 128]
+  float* part_ml;  // [n_split, B, Hk, R, 2]
+};
+
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2f(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// maximum that keeps a NaN (fmaxf drops it): a NaN score has to reach its row's output
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
+// D += A(16x16, row) * B(16x8, col), f16 inputs, fp32 accumulators
+__device__ __forceinline__ void mma16816_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// Codes (bytes 0, 1) and (bytes 2, 3) of a word as two f16 pairs. int8: a byte with its sign bit
+// flipped is u = code + 128, and 0x6400 | u is the f16 number 1024 + u, so one subtraction of 1152
+// gives the code exactly.
+template <int FMT>
+__device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (FMT == CACHE_INT8) {
+    const uint32_t u = w ^ 0x80808080u;
+    const __half2 off = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    __half2 ha = __hsub2(*reinterpret_cast<__half2*>(&a), off), hb = __hsub2(*reinterpret_cast<__half2*>(&b), off);
+    lo = *reinterpret_cast<uint32_t*>(&ha);
+    hi = *reinterpret_cast<uint32_t*>(&hb);
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(w));
+  }
+}
+
+// The queries of a warp's 8 * NT rows as B operands. Row r of the KV head is query token r / G,
+// head h * G + r % G; rows at or past R are zero.
+template <int NT>
+struct QueryFrag {
+  uint32_t b[NT][8][2];
+  float fac[NT][2];  // score factor of accumulator columns 2c, 2c+1: softmax scale * log2(e) / the row's power of two
+  int row[NT][2];    // rows of those columns
+};
+
+template <int NT>
+__device__ __forceinline__ void load_queries(QueryFrag<NT>& f, const DecArgs& a, int b, int h, int row0, int lane) {
+  const int g = lane >> 2, c = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    const int r = row0 + nt * 8 + g;
+    uint4 w[4] = {};
+    if (r < a.R) {
+      const uint4* p = reinterpret_cast<const uint4*>(a.q + b * a.q_b + (long long)(r / a.G) * a.q_tok +
+                                                      (long long)(h * a.G + r % a.G) * a.q_h + 32 * c);
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[i] = p[i];
+    }
+    const uint32_t* x = reinterpret_cast<const uint32_t*>(w);
+    uint32_t m2 = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i++) m2 = __vmaxu2(m2, x[i] & 0x7fff7fffu);
+    uint32_t m = max(m2 & 0xffffu, m2 >> 16);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    // bring the row's largest magnitude to 1 .. 4 by a power of two whose inverse is a normal
+    // number too; a row with NaN or infinity stays as it is
+    const int e = m >= 0x7f80u ? 0 : min(126, max(-126, (int)(m >> 7) - 127));
+    const float up = __int_as_float((127 - e) << 23), down = __int_as_float((127 + e) << 23);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const uint32_t y = x[2 * j + i];
+        __half2 hh = __floats2half2_rn(__uint_as_float(y << 16) * up, __uint_as_float(y & 0xffff0000u) * up);
+        f.b[nt][j][i] = *reinterpret_cast<uint32_t*>(&hh);
+      }
+    }
+    // the factors of columns 2c, 2c+1 live in the lanes of rows g = 2c, 2c+1
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      f.fac[nt][i] = __shfl_sync(0xffffffffu, down, (2 * c + i) * 4) * a.scale_log2;
+      f.row[nt][i] = row0 + nt * 8 + 2 * c + i;
+    }
+  }
+}
+
+// Running softmax of a warp: accumulators O^T (dims 16g + 2j (+1) x columns 2c (+1)), reference m
+// and this lane's part of the sum for the two columns.
+template <int NT>
+struct RowState {
+  float o[8][NT][4];
+  float m[NT][2], l[NT][2];
+};
+
+// One tile of KT keys: `kt`/`vt` give 16-byte pieces (row, piece) of the tile's codes, `lim` the
+// number of keys of the tile that each column sees (KT or more: all).
+template <int NT, int FMT, class KLoad, class VLoad>
+__device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT>& qf, KLoad kt, VLoad vt,
+                                            const float (&ks)[KT / 16], const float (&vs)[KT / 16],
+                                            const int (&lim)[NT][2], bool masked, int lane) {
+  const int g = lane >> 2, c = lane & 3;
+  constexpr int MT = KT / 16;
+  float s[MT][NT][4];
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
+#pragma unroll
+    for (int hh = 0; hh < 2; hh++) {
+      const uint4 x = kt(mt * 16 + g, 2 * c + hh), y = kt(mt * 16 + g + 8, 2 * c + hh);
+      const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        uint32_t a0, a1, a2, a3;
+        decode4<FMT>(xw[w], a0, a2);
+        decode4<FMT>(yw[w], a1, a3);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+          mma16816_f16(s[mt][nt], a0, a1, a2, a3, qf.b[nt][hh * 4 + w][0], qf.b[nt][hh * 4 + w][1]);
+      }
+    }
+  }
+  float lv[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++) lv[mt] = lg2f(fmaxf(vs[mt], 0x1p-100f));
+  uint32_t pb[MT][NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float z = s[mt][nt][e] * (ks[mt] * qf.fac[nt][e & 1]);
+        if (masked && mt * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1]) z = -INFINITY;
+        s[mt][nt][e] = z;
+        top[e & 1] = max_nan(top[e & 1], z + lv[mt]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 4));
+      top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 8));
+      top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
+      const float m_new = max_nan(st.m[nt][i], top[i]);
+      const float ref = m_new == -INFINITY ? 0.f : m_new;
+      const float al = st.m[nt][i] == -INFINITY ? 0.f : ex2f(st.m[nt][i] - ref);
+      st.m[nt][i] = m_new;
+      st.l[nt][i] *= al;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        st.o[j][nt][i] *= al;
+        st.o[j][nt][2 + i] *= al;
+      }
+      top[i] = ref;
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float p = ex2f(s[mt][nt][e] - top[e & 1]);
+        st.l[nt][e & 1] += p;
+        // a key that the column does not see weighs exactly 0, whatever its block's scale
+        w[e] = masked && mt * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1] ? 0.f : p * vs[mt];
+      }
+      __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+      pb[mt][nt][0] = transpose8x8(*reinterpret_cast<uint32_t*>(&h0));
+      pb[mt][nt][1] = transpose8x8(*reinterpret_cast<uint32_t*>(&h1));
+    }
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; mt++) {
+    const uint4 v0 = vt(mt * 16 + 2 * c, g), v1 = vt(mt * 16 + 2 * c + 1, g);
+    const uint4 v2 = vt(mt * 16 + 2 * c + 8, g), v3 = vt(mt * 16 + 2 * c + 9, g);
+    const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
+    const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w}, w3[4] = {v3.x, v3.y, v3.z, v3.w};
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
+      decode4<FMT>(__byte_perm(w0[w], w1[w], 0x5140), a0, a1);
+      decode4<FMT>(__byte_perm(w2[w], w3[w], 0x5140), a2, a3);
+      decode4<FMT>(__byte_perm(w0[w], w1[w], 0x7362), b0, b1);
+      decode4<FMT>(__byte_perm(w2[w], w3[w], 0x7362), b2, b3);
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        mma16816_f16(st.o[2 * w][nt], a0, a1, a2, a3, pb[mt][nt][0], pb[mt][nt][1]);
+        mma16816_f16(st.o[2 * w + 1][nt], b0, b1, b2, b3, pb[mt][nt][0], pb[mt][nt][1]);
+      }
+    }
+  }
+}
+
+template <int NT>
+struct DecSmem {
+  float o[NWARP][8 * NT][HD + 4];
+  float m[NWARP][8 * NT], l[NWARP][8 * NT];
+};
+
+__device__ __forceinline__ int seq_len(const DecArgs& a, int b) {
+  return max(0, min(a.kv_len ? a.kv_len[b] : a.len_all, a.max_len));
+}
+
+template <int NT, int FMT>
+__global__ void __launch_bounds__(32 * NWARP) cache_decode_kernel(DecArgs a) {
+  __shared__ DecSmem<NT> sm;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int split = blockIdx.x, h = blockIdx.y / a.n_group, row0 = (blockIdx.y % a.n_group) * 8 * NT, b = blockIdx.z;
+  const int len = seq_len(a, b);
+  const int tiles = (len + KT - 1) / KT;
+  const int t_begin = (int)((long long)tiles * split / a.n_split), t_end = (int)((long long)tiles * (split + 1) / a.n_split);
+  QueryFrag<NT> qf;
+  load_queries<NT>(qf, a, b, h, row0, lane);
+  RowState<NT> st;
+  int sees[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      st.m[nt][i] = -INFINITY;
+      st.l[nt][i] = 0.f;
+      sees[nt][i] = len - a.Sq + 1 + min(qf.row[nt][i], a.R - 1) / a.G;
+#pragma unroll
+      for (int j = 0; j < 8; j++) st.o[j][nt][i] = st.o[j][nt][2 + i] = 0.f;
+    }
+  }
+  const uint8_t* kb = a.k.codes + b * a.k.c_b + h * a.k.c_h;
+  const uint8_t* vb = a.v.codes + b * a.v.c_b + h * a.v.c_h;
+  for (int t = t_begin + warp; t < t_end; t += NWARP) {
+    const int key0 = t * KT;
+    float ks[KT / 16], vs[KT / 16];
+#pragma unroll
+    for (int i = 0; i < KT / 16; i++) {  // 16 keys never straddle a block; a tile's tail past the length reads the last block's
+      const long long blk = min(key0 + 16 * i, len - 1) >> a.block_shift;
+      ks[i] = a.k.scale[b * a.k.s_b + blk * a.k.s_blk + h * a.k.s_h];
+      vs[i] = a.v.scale[b * a.v.s_b + blk * a.v.s_blk + h * a.v.s_h];
+    }
+    int lim[NT][2];
+    bool masked = key0 + KT > len - a.Sq + 1;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) lim[nt][0] = sees[nt][0] - key0, lim[nt][1] = sees[nt][1] - key0;
+    // rows past the length repeat its last row: in bounds, and masked below
+    auto kt = [&](int r, int piece) {
+      return __ldg(reinterpret_cast<const uint4*>(kb + (long long)min(key0 + r, len - 1) * a.k.c_tok) + piece);
+    };
+    auto vt = [&](int r, int piece) {
+      return __ldg(reinterpret_cast<const uint4*>(vb + (long long)min(key0 + r, len - 1) * a.v.c_tok) + piece);
+    };
+    attend_tile<NT, FMT>(st, qf, kt, vt, ks, vs, lim, masked, lane);
+  }
+  // ---- merge the warps
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      float l = st.l[nt][i];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      const int n = nt * 8 + 2 * c + i;
+      if (g == 0) {
+        sm.m[warp][n] = st.m[nt][i];
+        sm.l[warp][n] = l;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        sm.o[warp][n][16 * g + 2 * j] = st.o[j][nt][i];
+        sm.o[warp][n][16 * g + 2 * j + 1] = st.o[j][nt][2 + i];
+      }
+    }
+  }
+  __syncthreads();
+  const int d = threadIdx.x;
+  for (int n = 0; n < 8 * NT; n++) {
+    const int r = row0 + n;
+    if (r >= a.R) break;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < NWARP; w++) M = max_nan(M, sm.m[w][n]);
+    float num = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 0; w < NWARP; w++) {
+      const float f = sm.m[w][n] == -INFINITY ? 0.f : ex2f(sm.m[w][n] - M);
+      num += f * sm.o[w][n][d];
+      den += f * sm.l[w][n];
+    }
+    if (a.n_split == 1) {
+      a.o[b * a.o_b + (long long)(r / a.G) * a.o_tok + (long long)(h * a.G + r % a.G) * a.o_h + d] =
+          __float2bfloat16(len - a.Sq + 1 + r / a.G <= 0 ? 0.f : num / den);
+    } else {
+      const long long row = (((long long)split * a.B + b) * a.Hk + h) * a.R + r;
+      a.part_o[row * HD + d] = num;
+      if (d == 0) {
+        a.part_ml[row * 2] = M;
+        a.part_ml[row * 2 + 1] = den;
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(HD) cache_combine_kernel(DecArgs a) {
+  const long long row = blockIdx.x;  // (b * Hk + h) * R + r
+  const int r = (int)(row % a.R), h = (int)(row / a.R % a.Hk), b = (int)(row / a.R / a.Hk), d = threadIdx.x;
+  const long long rows = (long long)a.B * a.Hk * a.R;
+  float M = -INFINITY;
+  for (int s = 0; s < a.n_split; s++) M = max_nan(M, a.part_ml[(s * rows + row) * 2]);
+  float num = 0.f, den = 0.f;
+  for (int s = 0; s < a.n_split; s++) {
+    const float m = a.part_ml[(s * rows + row) * 2];
+    if (m == -INFINITY) continue;
+    const float f = ex2f(m - M);
+    den += f * a.part_ml[(s * rows + row) * 2 + 1];
+    num += f * a.part_o[(s * rows + row) * HD + d];
+  }
+  a.o[b * a.o_b + (long long)(r / a.G) * a.o_tok + (long long)(h * a.G + r % a.G) * a.o_h + d] =
+      __float2bfloat16(seq_len(a, b) - a.Sq + 1 + r / a.G <= 0 ? 0.f : num / den);
+}
+
+int rows_of(const CacheDecodeProblem& p) { return p.Sq * (p.Hq / p.Hk); }
+int col_tiles(const CacheDecodeProblem& p) { return rows_of(p) > 8 ? 2 : 1; }
+int groups_of(const CacheDecodeProblem& p) { return (rows_of(p) + 8 * col_tiles(p) - 1) / (8 * col_tiles(p)); }
+
+// about four CTAs an SM, each with at least two tiles a warp
+int splits_of(const CacheDecodeProblem& p) {
+  const long long base = (long long)p.B * p.Hk * groups_of(p);
+  const int tiles = (p.max_len + KT - 1) / KT;
+  const long long n = (4LL * p.num_sms + base - 1) / base;
+  return (int)max(1LL, min(n, (long long)(tiles / (2 * NWARP))));
+}
+
+}  // namespace
+
+size_t cache_decode_scratch_floats(const CacheDecodeProblem& p) {
+  const int n = splits_of(p);
+  return n > 1 ? (size_t)n * p.B * p.Hk * rows_of(p) * (HD + 2) : 0;
+}
+
+int cache_decode_launches(const CacheDecodeProblem& p) { return splits_of(p) > 1 ? 2 : 1; }
+
+cudaError_t cache_append(const CacheAppendProblem& p, cudaStream_t stream) {
+  if (p.B <= 0 || p.S <= 0 || p.Hk <= 0) return cudaSuccess;
+  AppendArgs a;
+  a.B = p.B;
+  a.S = p.S;
+  a.Hk = p.Hk;
+  a.L = p.L;
+  for (int i = 0; i < 2; i++) {
+    a.x[i] = p.x[i];
+    a.x_b[i] = p.x_b[i];
+    a.x_tok[i] = p.x_tok[i];
+    a.x_h[i] = p.x_h[i];
+    a.side[i] = p.side[i];
+  }
+  a.pos = p.pos;
+  a.pos_all = p.pos_all;
+  a.n_new = p.n_new;
+  // blocks that S tokens can touch; a known position says exactly how many
+  a.n_rel = p.pos ? (p.S + p.block - 2) / p.block + 1 : (p.pos_all % p.block + p.S + p.block - 1) / p.block;
+  switch (p.block) {
+    case 16: return launch_append<16>(a, p.format, stream);
+    case 32: return launch_append<32>(a, p.format, stream);
+    case 64: return launch_append<64>(a, p.format, stream);
+    case 128: return launch_append<128>(a, p.format, stream);
+    case 256: return launch_append<256>(a, p.format, stream);
+  }
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream) {
+  if (p.B <= 0 || p.Sq <= 0 || p.Hq <= 0) return cudaSuccess;
+  if (p.Hk <= 0 || p.Hq % p.Hk) return cudaErrorInvalidValue;
+  DecArgs a;
+  a.B = p.B;
+  a.Sq = p.Sq;
+  a.Hq = p.Hq;
+  a.Hk = p.Hk;
+  a.L = p.L;
+  a.G = p.Hq / p.Hk;
+  a.R = rows_of(p);
+  a.n_group = groups_of(p);
+  a.block_shift = 31 - __builtin_clz((unsigned)p.block);
+  a.q = p.q;
+  a.q_b = p.q_b;
+  a.q_tok = p.q_tok;
+  a.q_h = p.q_h;
+  a.o = p.o;
+  a.o_b = p.o_b;
+  a.o_tok = p.o_tok;
+  a.o_h = p.o_h;
+  a.k = p.side[0];
+  a.v = p.side[1];
+  a.kv_len = p.kv_len;
+  a.len_all = p.len_all;
+  a.max_len = p.max_len;
+  a.scale_log2 = p.scale * 1.4426950408889634f;
+  a.n_split = splits_of(p);
+  const long long rows = (long long)p.B * p.Hk * a.R;
+  if (rows > 0x7fffffffLL || p.B > 65535 || (long long)p.Hk * a.n_group > 65535) return cudaErrorInvalidValue;
+  if (a.n_split > 1 && p.scratch == nullptr) return cudaErrorInvalidValue;
+  a.part_o = p.scratch;
+  a.part_ml = p.scratch ? p.scratch + (size_t)a.n_split * rows * HD : nullptr;
+  const dim3 grid(a.n_split, p.Hk * a.n_group, p.B);
+  const bool i8 = p.format == CACHE_INT8;
+  if (col_tiles(p) == 1) {
+    if (i8) cache_decode_kernel<1, CACHE_INT8><<<grid, 32 * NWARP, 0, stream>>>(a);
+    else cache_decode_kernel<1, CACHE_E4M3><<<grid, 32 * NWARP, 0, stream>>>(a);
+  } else {
+    if (i8) cache_decode_kernel<2, CACHE_INT8><<<grid, 32 * NWARP, 0, stream>>>(a);
+    else cache_decode_kernel<2, CACHE_E4M3><<<grid, 32 * NWARP, 0, stream>>>(a);
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || a.n_split == 1) return e;
+  cache_combine_kernel<<<(unsigned)rows, HD, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace ft
