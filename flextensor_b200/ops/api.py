@@ -191,6 +191,28 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     return out
 
 
+MOE_DECODE_MAX_TOKENS = 64
+
+
+def moe_decode(x: torch.Tensor, router: torch.Tensor, w_gate_up, w_down, topk: int, *,
+               residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A whole mixture-of-experts feed-forward for at most 64 tokens (a decode step), with no
+    synchronisation with the host: ``out = residual + sum_k w_k * down_k(swiglu(gate_up_k(x)))``.
+
+    ``x [T, D]``, ``router [E, D]`` (at most 128 experts); ``w_gate_up`` / ``w_down``: a sequence of one
+    ``[2F, D]`` (gate and up rows interleaved) / ``[D, F]`` tensor per expert, or one stacked tensor.
+    Each token takes the ``topk`` (at most 8) experts of the largest router logits (fp32; equal ones
+    go to the lower index) weighted by the softmax over those. ``out`` may be ``residual`` or ``x``."""
+    if isinstance(w_gate_up, torch.Tensor):
+        w_gate_up = w_gate_up.unbind(0)
+    if isinstance(w_down, torch.Tensor):
+        w_down = w_down.unbind(0)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _count(native.lib().moe_decode(x, router, w_gate_up, w_down, topk, residual, out))
+    return out
+
+
 def attention_cp(q: torch.Tensor, kv_local: torch.Tensor, *, peer_kv: list[int], flags_ptr: int, flag_stride: int,
                  peer_acks: list[int], rank: int, shard_rows: int, epoch: int, counters: torch.Tensor,
                  scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:

@@ -27,6 +27,7 @@ SOURCES = [
     "moe_sm100.cu",
     "decode_sm100.cu",
     "cache_q8_sm100.cu",
+    "moe_decode_sm100.cu",
 ]
 
 CUDA_FLAGS = [

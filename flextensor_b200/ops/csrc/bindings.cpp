@@ -16,6 +16,7 @@
 #include "ft_runtime.h"
 #include "ft_tp.h"
 #include "ft_moe.h"
+#include "ft_moe_decode.h"
 
 namespace {
 
@@ -432,6 +433,74 @@ int64_t decode_attention_q8(const Tensor& q_in, const Tensor& kc, const Tensor& 
   return ft::cache_decode_launches(p);
 }
 
+// returns the number of kernels launched
+int64_t moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tensor>& gate_up,
+                   const std::vector<Tensor>& down, int64_t topk, const c10::optional<Tensor>& residual, Tensor& out) {
+  const char* op = "moe_decode";
+  auto matrix = [&](const Tensor& t, const char* name, int64_t r, int64_t c) {
+    TORCH_CHECK(t.scalar_type() == at::kBFloat16, op, ": ", name, " must be bfloat16");
+    TORCH_CHECK(t.dim() == 2 && t.size(0) == r && t.size(1) == c, op, ": ", name, " must be [", r, ", ", c, "], got ",
+                t.sizes());
+    TORCH_CHECK(t.stride(1) == 1 && t.stride(0) % 8 == 0 && on_16_bytes(t), op, ": rows of ", name,
+                " must be contiguous and start on 16-byte boundaries");
+  };
+  TORCH_CHECK(x.dim() == 2 && router.dim() == 2, op, ": x must be [T, D] and router [E, D], got ", x.sizes(), " and ",
+              router.sizes());
+  const int64_t T = x.size(0), D = x.size(1), E = router.size(0);
+  TORCH_CHECK(T <= ft::kMoeDecMaxTokens, op, ": at most ", ft::kMoeDecMaxTokens, " tokens, got ", T);
+  TORCH_CHECK(E >= 1 && E <= ft::kMoeDecMaxExperts, op, ": 1 to ", ft::kMoeDecMaxExperts, " experts, got ", E);
+  TORCH_CHECK(topk >= 1 && topk <= ft::kMoeDecMaxTopk && topk <= E, op, ": topk must lie in [1, min(E, ",
+              ft::kMoeDecMaxTopk, ")], got ", topk);
+  TORCH_CHECK((int64_t)gate_up.size() == E && (int64_t)down.size() == E, op, ": one w_gate_up and one w_down per expert (",
+              E, "), got ", gate_up.size(), " and ", down.size());
+  TORCH_CHECK(down[0].dim() == 2, op, ": w_down must be [D, F] per expert");
+  const int64_t F = down[0].size(1);
+  TORCH_CHECK(D >= 8 && D % 8 == 0 && F >= 8 && F % 8 == 0 && D < (1 << 20) && F < (1 << 20), op,
+              ": D and F must be multiples of 8, got ", D, " and ", F);
+  matrix(x, "x", T, D);
+  matrix(router, "router", E, D);
+  matrix(out, "out", T, D);
+  const bool res = residual && residual->defined();
+  if (res) matrix(*residual, "residual", T, D);
+  ft::MoeDecodeProblem p;
+  for (int64_t e = 0; e < E; e++) {
+    matrix(gate_up[e], "w_gate_up", 2 * F, D);
+    matrix(down[e], "w_down", D, F);
+    TORCH_CHECK(gate_up[e].stride(0) == gate_up[0].stride(0) && down[e].stride(0) == down[0].stride(0), op,
+                ": the experts' weights must have one row stride");
+    p.w_gate_up[e] = reinterpret_cast<const __nv_bfloat16*>(gate_up[e].data_ptr());
+    p.w_down[e] = reinterpret_cast<const __nv_bfloat16*>(down[e].data_ptr());
+  }
+  TORCH_CHECK(at::has_internal_overlap(out) != at::MemOverlap::Yes, op, ": out must not overlap itself");
+  at::assert_no_partial_overlap(out, x);
+  if (res) at::assert_no_partial_overlap(out, *residual);
+  check_same_cuda(x, {&router, &out}, op);
+  if (res) check_same_cuda(x, {&*residual}, op);
+  for (int64_t e = 0; e < E; e++) check_same_cuda(x, {&gate_up[e], &down[e]}, op);
+  if (T == 0) return 0;
+  c10::cuda::CUDAGuard g(x.device());
+  p.T = (int)T;
+  p.D = (int)D;
+  p.F = (int)F;
+  p.E = (int)E;
+  p.topk = (int)topk;
+  p.x = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
+  p.ldx = x.stride(0);
+  p.router = reinterpret_cast<const __nv_bfloat16*>(router.data_ptr());
+  p.ldr = router.stride(0);
+  p.ld_gate_up = gate_up[0].stride(0);
+  p.ld_down = down[0].stride(0);
+  p.residual = reinterpret_cast<const __nv_bfloat16*>(opt_ptr(residual));
+  p.ldres = res ? residual->stride(0) : 0;
+  p.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  p.ldo = out.stride(0);
+  p.num_sms = num_sms_for(x.get_device());
+  Tensor ws = at::empty({(int64_t)ft::moe_decode_workspace(p)}, x.options().dtype(at::kByte));
+  p.workspace = ws.data_ptr();
+  check_ok(ft::moe_decode(p, at::cuda::getCurrentCUDAStream()), op);
+  return ft::moe_decode_launches(p);
+}
+
 void attention_cp(const Tensor& q, const Tensor& kv_local, Tensor& o, double scale, std::vector<uint64_t> peer_kv,
                   uint64_t flags, int64_t flag_stride, std::vector<uint64_t> peer_acks, int64_t rank,
                   int64_t shard_rows, uint64_t epoch, Tensor& counters) {
@@ -793,7 +862,7 @@ int device_error(bool reset) {
   int m = ft::moe_device_error(reset);
   int d = ft::decode_device_error(reset);
   int c = ft::cache_device_error(reset);
-  return e ? e : (n ? n : (a ? a : (p ? p : (t ? t : (m ? m : (d ? d : c))))));
+  return e ? e : (n ? n : (a ? a : (p ? p : (t ? t : (m ? m : (d ? d : (c ? c : ft::moe_decode_device_error(reset))))))));
 }
 
 struct PyEngine {
@@ -904,6 +973,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention_q8", &decode_attention_q8, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("k_scale"), py::arg("v_scale"), py::arg("out"), py::arg("kv_len"), py::arg("len_all"),
         py::arg("max_len"), py::arg("block"), py::arg("scale"));
+  m.def("moe_decode", &moe_decode, py::arg("x"), py::arg("router"), py::arg("w_gate_up"), py::arg("w_down"),
+        py::arg("topk"), py::arg("residual"), py::arg("out"));
   m.def("p2p_publish_raw", &p2p_publish_raw);
   m.def("tp_ag_gemm", &tp_ag_gemm, py::arg("a_full"), py::arg("w"), py::arg("out"), py::arg("bias"), py::arg("epi"),
         py::arg("peer_a"), py::arg("flags"), py::arg("flag_stride"), py::arg("peer_acks"), py::arg("rank"),

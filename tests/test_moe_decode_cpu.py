@@ -1,0 +1,87 @@
+"""Refusals of ``ops.moe_decode`` (checked before the device, so on CPU tensors), and a model in
+Python of how its products divide the stream of weight tiles among CTAs."""
+
+import random
+
+import pytest
+import torch
+
+from flextensor_b200 import ops
+from flextensor_b200.ops import native
+
+T, D, F, E = 3, 64, 32, 4
+
+
+def args(t=T, d=D, f=F, e=E):
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    return dict(x=z(t, d), router=z(e, d), w_gate_up=[z(2 * f, d) for _ in range(e)], w_down=[z(d, f) for _ in range(e)], topk=2)
+
+
+def bf(*s):
+    return torch.zeros(*s, dtype=torch.bfloat16)
+
+
+@pytest.mark.skipif(not native.available(), reason="native extension not built")
+@pytest.mark.parametrize("change,match", [
+    ({}, "CUDA device"),
+    (dict(x=torch.zeros(T, D)), "x must be bfloat16"),
+    (dict(x=bf(T, D, 1)), r"x must be \[T, D\]"),
+    (dict(x=bf(65, D)), "at most 64 tokens"),
+    (dict(router=bf(E, D + 8)), "router must be"),
+    (dict(router=bf(0, D)), "experts"),
+    (dict(topk=0), "topk"),
+    (dict(topk=5), "topk"),
+    (dict(w_down=[bf(D, F)] * 3), "one w_gate_up and one w_down"),
+    (dict(w_gate_up=[bf(2 * F, D)] * 3 + [bf(2 * F + 2, D)]), "w_gate_up must be"),
+    (dict(w_gate_up=[bf(2 * F, D)] * 3 + [bf(2 * F, D).float()]), "w_gate_up must be"),
+    (dict(w_gate_up=[bf(2 * F, D)] * 3 + [bf(2 * F, 2 * D)[:, :D]]), "one row stride"),
+    (dict(w_down=[bf(D, F)] * 3 + [bf(F, D).t()]), "16-byte"),
+    (dict(w_down=[bf(D, F)] * 3 + [bf(D * F + 1)[1:].view(D, F)]), "16-byte"),
+    (dict(residual=bf(T, D + 8)), "residual must be"),
+    (dict(out=bf(T + 1, D)), "out must be"),
+    (dict(out=bf(1, D).expand(T, D)), "overlap"),
+])
+def test_refusals(change, match):
+    a = args()
+    a.update(change)
+    with pytest.raises(RuntimeError, match=match):
+        ops.moe_decode(**a)
+
+
+@pytest.mark.skipif(not native.available(), reason="native extension not built")
+def test_refuses_odd_sizes_and_partial_overlap():
+    with pytest.raises(RuntimeError, match="multiples of 8"):
+        ops.moe_decode(**args(d=60))
+    with pytest.raises(RuntimeError, match="multiples of 8"):
+        ops.moe_decode(**args(f=36))
+    buf = bf(T + 1, D)
+    with pytest.raises(RuntimeError, match="overlap|memory"):
+        ops.moe_decode(**dict(args(), residual=buf[:T], out=buf[1:]))
+
+
+def splits(D_, F_, topk, sms, min_chunks=4):
+    rt, kc = -(-D_ // 128), -(-F_ // 64)
+    m = max(min_chunks, rt * kc * topk // sms)
+    return (kc - 1 + m - 1) // m + 1
+
+
+def test_stream_partition_model():
+    """Runs cover the stream once, a run cuts at most two tiles, ``owner`` finds the run of a tile, and
+    the number of CTAs on one row tile stays within what the workspace holds."""
+    rng = random.Random(0)
+    for _ in range(400):
+        D_, F_, topk = 8 * rng.randint(1, 800), 8 * rng.randint(1, 2100), rng.randint(1, 8)
+        n_act, sms = rng.randint(topk, 64), rng.choice([148, 132, 7])
+        rt, kc = -(-D_ // 128), -(-F_ // 64)
+        total = n_act * rt * kc
+        ctas = min(sms, max(1, total // 4))
+        begin = lambda c: total * c // ctas  # noqa: E731
+        owner = lambda i: ((i + 1) * ctas - 1) // total  # noqa: E731
+        assert begin(0) == 0 and begin(ctas) == total
+        for c in range(ctas):
+            assert begin(c) < begin(c + 1) and owner(begin(c)) == c == owner(begin(c + 1) - 1)
+        for it in [rng.randrange(n_act * rt) for _ in range(20)]:
+            c0, c1 = owner(it * kc), owner((it + 1) * kc - 1)
+            assert c1 - c0 + 1 <= splits(D_, F_, topk, sms)
+            for c in range(c0, c1 + 1 if c1 > c0 else c0):  # a tile that several share is each one's first or last
+                assert begin(c) // kc == it or (begin(c + 1) - 1) // kc == it
