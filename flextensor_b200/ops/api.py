@@ -180,14 +180,13 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     bounds it: longer ones are cut)."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if isinstance(kv_len, torch.Tensor):
         ml = k_cache.shape[1] if max_len is None else max_len
-        n = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, kv_len, 0, ml, block, scale)
+        out = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, kv_len, 0, ml, block, scale)
     else:
-        n = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, None, kv_len, kv_len, block, scale)
-    _count(n)
+        out = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, None, kv_len, kv_len, block,
+                                               scale)
+    _count(2)
     return out
 
 
@@ -207,9 +206,8 @@ def moe_decode(x: torch.Tensor, router: torch.Tensor, w_gate_up, w_down, topk: i
         w_gate_up = w_gate_up.unbind(0)
     if isinstance(w_down, torch.Tensor):
         w_down = w_down.unbind(0)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _count(native.lib().moe_decode(x, router, w_gate_up, w_down, topk, residual, out))
+    out = native.lib().moe_decode(x, router, w_gate_up, w_down, topk, residual, out)
+    _count(4)
     return out
 
 

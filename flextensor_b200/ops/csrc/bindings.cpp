@@ -380,15 +380,15 @@ void kv_append_q8(const Tensor& k, const Tensor& v, Tensor& kc, Tensor& vc, Tens
   check_ok(ft::cache_append(p, at::cuda::getCurrentCUDAStream()), op);
 }
 
-// returns the number of kernels launched
-int64_t decode_attention_q8(const Tensor& q_in, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
-                            Tensor& o_in, const c10::optional<Tensor>& kv_len, int64_t len_all, int64_t max_len,
-                            int64_t block, double scale) {
+Tensor decode_attention_q8(const Tensor& q_in, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
+                           const c10::optional<Tensor>& o_given, const c10::optional<Tensor>& kv_len, int64_t len_all,
+                           int64_t max_len, int64_t block, double scale) {
   const char* op = "decode_attention_q8";
   check_cache(kc, vc, ks, vs, block, op);
   const Tensor q = q_in.dim() == 3 ? q_in.unsqueeze(1) : q_in;
-  const Tensor o = o_in.dim() == 3 ? o_in.unsqueeze(1) : o_in;
   check_rows(q, op, "q");
+  const Tensor o_in = o_given && o_given->defined() ? *o_given : at::empty(q_in.sizes(), q_in.options());
+  const Tensor o = o_in.dim() == 3 ? o_in.unsqueeze(1) : o_in;
   check_rows(o, op, "out");
   const int64_t B = kc.size(0), L = kc.size(1), Hk = kc.size(2), Sq = q.size(1), Hq = q.size(2);
   TORCH_CHECK(q.size(0) == B, op, ": q has ", q.size(0), " sequences, the cache ", B);
@@ -424,18 +424,16 @@ int64_t decode_attention_q8(const Tensor& q_in, const Tensor& kc, const Tensor& 
   p.max_len = (int)(each ? max_len : len_all);
   p.scale = (float)scale;
   p.num_sms = num_sms_for(kc.get_device());
-  Tensor scratch;
-  if (const size_t n = ft::cache_decode_scratch_floats(p)) {
-    scratch = at::empty({(int64_t)n}, ks.options());
-    p.scratch = scratch.data_ptr<float>();
-  }
+  if (q.numel() == 0) return o_in;
+  const Tensor scratch = at::empty({(int64_t)ft::cache_decode_scratch_floats(p)}, ks.options());
+  p.scratch = scratch.data_ptr<float>();
   check_ok(ft::cache_decode(p, at::cuda::getCurrentCUDAStream()), op);
-  return ft::cache_decode_launches(p);
+  return o_in;
 }
 
-// returns the number of kernels launched
-int64_t moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tensor>& gate_up,
-                   const std::vector<Tensor>& down, int64_t topk, const c10::optional<Tensor>& residual, Tensor& out) {
+Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tensor>& gate_up,
+                  const std::vector<Tensor>& down, int64_t topk, const c10::optional<Tensor>& residual,
+                  const c10::optional<Tensor>& out_given) {
   const char* op = "moe_decode";
   auto matrix = [&](const Tensor& t, const char* name, int64_t r, int64_t c) {
     TORCH_CHECK(t.scalar_type() == at::kBFloat16, op, ": ", name, " must be bfloat16");
@@ -459,6 +457,7 @@ int64_t moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tens
               ": D and F must be multiples of 8, got ", D, " and ", F);
   matrix(x, "x", T, D);
   matrix(router, "router", E, D);
+  const Tensor out = out_given && out_given->defined() ? *out_given : at::empty({T, D}, x.options());
   matrix(out, "out", T, D);
   const bool res = residual && residual->defined();
   if (res) matrix(*residual, "residual", T, D);
@@ -477,7 +476,7 @@ int64_t moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tens
   check_same_cuda(x, {&router, &out}, op);
   if (res) check_same_cuda(x, {&*residual}, op);
   for (int64_t e = 0; e < E; e++) check_same_cuda(x, {&gate_up[e], &down[e]}, op);
-  if (T == 0) return 0;
+  if (T == 0) return out;
   c10::cuda::CUDAGuard g(x.device());
   p.T = (int)T;
   p.D = (int)D;
@@ -498,7 +497,7 @@ int64_t moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tens
   Tensor ws = at::empty({(int64_t)ft::moe_decode_workspace(p)}, x.options().dtype(at::kByte));
   p.workspace = ws.data_ptr();
   check_ok(ft::moe_decode(p, at::cuda::getCurrentCUDAStream()), op);
-  return ft::moe_decode_launches(p);
+  return out;
 }
 
 void attention_cp(const Tensor& q, const Tensor& kv_local, Tensor& o, double scale, std::vector<uint64_t> peer_kv,

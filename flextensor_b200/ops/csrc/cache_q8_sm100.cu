@@ -21,16 +21,25 @@
 //      interleaved with PRMT into the (key, key+1) pairs the MMA wants.
 // P goes from the accumulator layout to the B operand with one 8x8 transpose per 8 keys.
 //
+// Work. All (sequence, KV head, row group) units form one sequence of 32-key tiles, divided into
+// equal contiguous runs, one per warp (8 warps an SM), so ragged batches and few long sequences load
+// every SM alike. A warp streams its run by itself through its own three 8 KB stages (TMA, 128-byte
+// swizzle; the warp's own program order says when a stage is free, so there is no producer and no
+// barrier between warps) and writes fp32 partial results at unit ends; a second kernel, launched
+// so that its start overlaps the first one's end, merges the partials of each row in run order.
+//
 // Scales: a score is (q . codes) * ks, and the weight of a value's codes is p * vs. The running
 // reference m is the maximum of score + log2(vs), so p * vs <= 1 whatever the scales are and f16
 // holds it to 2^-11 of the largest weight; the sum l takes p itself in fp32. q is scaled by a power
 // of two per row into f16 (exact but for elements below 2^-24 of the row's largest).
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
 #include "ft_cache.h"
+#include "ft_ops.h"
 #include "sm100_common.cuh"
 
 namespace ft {
@@ -177,23 +186,29 @@ cudaError_t launch_append(const AppendArgs& a, int format, cudaStream_t stream) 
 }
 
 // ------------------------------------------------------------------------------------ attention
-constexpr int KT = 32;   // keys of a warp's tile
-constexpr int NWARP = 4;
+constexpr int KT = 32;       // keys of a tile
+constexpr int NWARP = 8;
+constexpr int STAGES = 3;    // per warp
+constexpr int SIDE_BYTES = KT * HD;
+constexpr int STAGE_BYTES = 2 * SIDE_BYTES;  // keys, values
+constexpr int MERGE_WARPS = 8;
 
 struct DecArgs {
-  int B, Sq, Hq, Hk, L, G, R, n_group;  // R = Sq * G query rows of a KV head; n_group column groups of 8 * NT rows
+  int B, Sq, Hq, Hk, L, G, R, n_group;  // R = Sq * G query rows of a KV head in n_group groups of 8 * NT
   int block_shift;
+  int runs;                             // warps that may take a run
   const __nv_bfloat16* q;
   long long q_b, q_tok, q_h;
   __nv_bfloat16* o;
   long long o_b, o_tok, o_h;
   CacheSide k, v;
+  int one_b[2], one_h[2];               // keys / values: the cache is broadcast over sequences / heads (stride 0)
   const int* kv_len;
   int len_all, max_len;
-  float scale_log2;  // softmax scale * log2(e)
-  int n_split;
-  float* part_o;   // [n_split, B, Hk, R, 128]
-  float* part_ml;  // [n_split, B, Hk, R, 2]
+  float scale_log2;                     // softmax scale * log2(e)
+  float* part_o;                        // [units + runs][8 * NT][128]
+  float2* part_ml;                      // [units + runs][8 * NT] reference and sum
+  int merge_per_row;                    // warps that share a row of the merge
 };
 
 __device__ __forceinline__ float ex2f(float x) {
@@ -406,151 +421,377 @@ __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT
   }
 }
 
-template <int NT>
-struct DecSmem {
-  float o[NWARP][8 * NT][HD + 4];
-  float m[NWARP][8 * NT], l[NWARP][8 * NT];
+__device__ __forceinline__ int seq_len(const DecArgs& a, int b) {
+  return max(0, min(a.kv_len ? __ldg(a.kv_len + b) : a.len_all, a.max_len));
+}
+__device__ __forceinline__ int seq_tiles(const DecArgs& a, int b) { return (seq_len(a, b) + KT - 1) / KT; }
+
+// sum of the tiles of sequences [0, end) of one KV head and row group, by a whole warp
+__device__ __forceinline__ long long tiles_before(const DecArgs& a, int end, int lane) {
+  if (a.kv_len == nullptr) return (long long)end * seq_tiles(a, 0);
+  long long sum = 0;
+  for (int b = lane; b < end; b += 32) sum += seq_tiles(a, b);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum;
+}
+
+// The sequence of tiles and its division into runs.
+struct Runs {
+  long long total;
+  int n;
+  __device__ __forceinline__ Runs(long long t, int most) : total(t), n((int)min((long long)most, t)) {}
+  __device__ __forceinline__ long long begin(int r) const { return total * r / n; }
+  __device__ __forceinline__ int owner(long long i) const { return (int)(((i + 1) * n - 1) / total); }
 };
 
-__device__ __forceinline__ int seq_len(const DecArgs& a, int b) {
-  return max(0, min(a.kv_len ? a.kv_len[b] : a.len_all, a.max_len));
+// A place in the sequence of tiles.
+struct Cursor {
+  int b, hg, t, n;  // sequence, head * n_group + group, tile of the unit, tiles of a unit of this sequence
+  __device__ __forceinline__ void next(const DecArgs& a) {
+    if (++t < n) return;
+    t = 0;
+    if (++hg < a.Hk * a.n_group) return;
+    hg = 0;
+    do {
+      if (++b >= a.B) return;
+      n = seq_tiles(a, b);
+    } while (n == 0);
+  }
+};
+
+// the place of tile i, by a whole warp
+__device__ __forceinline__ Cursor locate(const DecArgs& a, long long i, int lane) {
+  Cursor c;
+  const int per = a.Hk * a.n_group;
+  if (a.kv_len == nullptr) {
+    c.n = seq_tiles(a, 0);
+    c.b = (int)(i / ((long long)c.n * per));
+    i -= (long long)c.b * c.n * per;
+  } else {
+    long long before = 0;
+    for (int b0 = 0;; b0 += 32) {  // i lies before the total, so some sequence holds it
+      const int n = b0 + lane < a.B ? seq_tiles(a, b0 + lane) : 0;
+      long long end = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, end, o);
+        if (lane >= o) end += up;
+      }
+      const unsigned int hit = __ballot_sync(0xffffffffu, (before + end) * per > i);
+      if (hit || b0 + 32 >= a.B) {
+        const int at = hit ? __ffs(hit) - 1 : 31;
+        c.b = b0 + at;
+        c.n = __shfl_sync(0xffffffffu, n, at);
+        i -= (before + __shfl_sync(0xffffffffu, end - n, at)) * per;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, end, 31);
+    }
+  }
+  c.hg = (int)(i / c.n);
+  c.t = (int)(i % c.n);
+  return c;
+}
+
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+
+// A wait that runs out (2 s) is recorded and answered with false.
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t phase) {
+  const uint32_t a = smem_u32(bar);
+  if (mbar_try_wait(a, phase)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(a, phase)) {
+    if ((unsigned long long)(clock64() - t0) > FT_WAIT_LIMIT_CYCLES) {
+      record_error(kErrWaitTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+struct DecSmem {
+  uint8_t stage[NWARP][STAGES][STAGE_BYTES];
+  uint64_t full[NWARP][STAGES];
+};
+
+struct TileScales {
+  float k[KT / 16], v[KT / 16];
+};
+
+// 16 keys never straddle a block; a tile's tail past the length takes the last block's scale
+__device__ __forceinline__ TileScales load_scales(const DecArgs& a, const Cursor& c) {
+  TileScales s;
+  const int h = c.hg / a.n_group, last = seq_len(a, c.b) - 1;
+#pragma unroll
+  for (int i = 0; i < KT / 16; i++) {
+    const long long blk = min(c.t * KT + 16 * i, last) >> a.block_shift;
+    s.k[i] = __ldg(a.k.scale + c.b * a.k.s_b + blk * a.k.s_blk + h * a.k.s_h);
+    s.v[i] = __ldg(a.v.scale + c.b * a.v.s_b + blk * a.v.s_blk + h * a.v.s_h);
+  }
+  return s;
 }
 
 template <int NT, int FMT>
-__global__ void __launch_bounds__(32 * NWARP) cache_decode_kernel(DecArgs a) {
-  __shared__ DecSmem<NT> sm;
+__global__ void __launch_bounds__(32 * NWARP, 1)
+    cache_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, DecArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  DecSmem& sm = *reinterpret_cast<DecSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int split = blockIdx.x, h = blockIdx.y / a.n_group, row0 = (blockIdx.y % a.n_group) * 8 * NT, b = blockIdx.z;
-  const int len = seq_len(a, b);
-  const int tiles = (len + KT - 1) / KT;
-  const int t_begin = (int)((long long)tiles * split / a.n_split), t_end = (int)((long long)tiles * (split + 1) / a.n_split);
+  pdl_launch();
+  const Runs runs(tiles_before(a, a.B, lane) * a.Hk * a.n_group, a.runs);
+  const int run = warp * gridDim.x + blockIdx.x;  // neighbouring runs on different SMs: few runs spread out
+  if (run >= runs.n) return;
+  const long long first = runs.begin(run);
+  const int n = (int)(runs.begin(run + 1) - first);
+  uint64_t* const full = sm.full[warp];
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; s++) mbar_init(&full[s], 1);
+    fence_barrier_init();
+  }
+  __syncwarp();
+  Cursor at = locate(a, first, lane), ahead = at;
+  auto fetch = [&](int s) {  // one lane: the tile at `ahead` into stage s
+    const int h = ahead.hg / a.n_group, key0 = ahead.t * KT;
+    uint8_t* const dst = sm.stage[warp][s];
+    mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
+    tma_load_4d(dst, &tm_k, &full[s], 0, a.one_h[0] ? 0 : h, key0, a.one_b[0] ? 0 : ahead.b);
+    tma_load_4d(dst + SIDE_BYTES, &tm_v, &full[s], 0, a.one_h[1] ? 0 : h, key0, a.one_b[1] ? 0 : ahead.b);
+  };
+  for (int s = 0; s < STAGES && s < n; s++) {
+    if (lane == 0) fetch(s);
+    ahead.next(a);
+  }
   QueryFrag<NT> qf;
-  load_queries<NT>(qf, a, b, h, row0, lane);
   RowState<NT> st;
-  int sees[NT][2];
+  int sees[NT][2], len = 0;
+  auto enter = [&]() {  // a new unit: its queries, empty accumulators
+    len = seq_len(a, at.b);
+    load_queries<NT>(qf, a, at.b, at.hg / a.n_group, at.hg % a.n_group * 8 * NT, lane);
 #pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
+    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-      st.m[nt][i] = -INFINITY;
-      st.l[nt][i] = 0.f;
-      sees[nt][i] = len - a.Sq + 1 + min(qf.row[nt][i], a.R - 1) / a.G;
+      for (int i = 0; i < 2; i++) {
+        st.m[nt][i] = -INFINITY;
+        st.l[nt][i] = 0.f;
+        sees[nt][i] = len - a.Sq + 1 + min(qf.row[nt][i], a.R - 1) / a.G;
 #pragma unroll
-      for (int j = 0; j < 8; j++) st.o[j][nt][i] = st.o[j][nt][2 + i] = 0.f;
-    }
-  }
-  const uint8_t* kb = a.k.codes + b * a.k.c_b + h * a.k.c_h;
-  const uint8_t* vb = a.v.codes + b * a.v.c_b + h * a.v.c_h;
-  for (int t = t_begin + warp; t < t_end; t += NWARP) {
-    const int key0 = t * KT;
-    float ks[KT / 16], vs[KT / 16];
-#pragma unroll
-    for (int i = 0; i < KT / 16; i++) {  // 16 keys never straddle a block; a tile's tail past the length reads the last block's
-      const long long blk = min(key0 + 16 * i, len - 1) >> a.block_shift;
-      ks[i] = a.k.scale[b * a.k.s_b + blk * a.k.s_blk + h * a.k.s_h];
-      vs[i] = a.v.scale[b * a.v.s_b + blk * a.v.s_blk + h * a.v.s_h];
-    }
-    int lim[NT][2];
-    bool masked = key0 + KT > len - a.Sq + 1;
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) lim[nt][0] = sees[nt][0] - key0, lim[nt][1] = sees[nt][1] - key0;
-    // rows past the length repeat its last row: in bounds, and masked below
-    auto kt = [&](int r, int piece) {
-      return __ldg(reinterpret_cast<const uint4*>(kb + (long long)min(key0 + r, len - 1) * a.k.c_tok) + piece);
-    };
-    auto vt = [&](int r, int piece) {
-      return __ldg(reinterpret_cast<const uint4*>(vb + (long long)min(key0 + r, len - 1) * a.v.c_tok) + piece);
-    };
-    attend_tile<NT, FMT>(st, qf, kt, vt, ks, vs, lim, masked, lane);
-  }
-  // ---- merge the warps
-#pragma unroll
-  for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      float l = st.l[nt][i];
-      l += __shfl_xor_sync(0xffffffffu, l, 4);
-      l += __shfl_xor_sync(0xffffffffu, l, 8);
-      l += __shfl_xor_sync(0xffffffffu, l, 16);
-      const int n = nt * 8 + 2 * c + i;
-      if (g == 0) {
-        sm.m[warp][n] = st.m[nt][i];
-        sm.l[warp][n] = l;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        sm.o[warp][n][16 * g + 2 * j] = st.o[j][nt][i];
-        sm.o[warp][n][16 * g + 2 * j + 1] = st.o[j][nt][2 + i];
+        for (int j = 0; j < 8; j++) st.o[j][nt][i] = st.o[j][nt][2 + i] = 0.f;
       }
     }
-  }
-  __syncthreads();
-  const int d = threadIdx.x;
-  for (int n = 0; n < 8 * NT; n++) {
-    const int r = row0 + n;
-    if (r >= a.R) break;
-    float M = -INFINITY;
+  };
+  enter();
+  TileScales sc = load_scales(a, at);
+  bool ok = true;
+  int s = 0;
+  uint32_t ph = 0;
+  for (int i = 0; i < n; i++) {
+    Cursor then = at;
+    then.next(a);
+    const TileScales sc_next = i + 1 < n ? load_scales(a, then) : sc;
+    if (ok) ok = __all_sync(0xffffffffu, bounded_wait(&full[s], ph));
+    if (ok) {
+      const int key0 = at.t * KT;
+      const uint32_t kb = smem_u32(sm.stage[warp][s]), vb = kb + SIDE_BYTES;
+      int lim[NT][2];
 #pragma unroll
-    for (int w = 0; w < NWARP; w++) M = max_nan(M, sm.m[w][n]);
-    float num = 0.f, den = 0.f;
-#pragma unroll
-    for (int w = 0; w < NWARP; w++) {
-      const float f = sm.m[w][n] == -INFINITY ? 0.f : ex2f(sm.m[w][n] - M);
-      num += f * sm.o[w][n][d];
-      den += f * sm.l[w][n];
-    }
-    if (a.n_split == 1) {
-      a.o[b * a.o_b + (long long)(r / a.G) * a.o_tok + (long long)(h * a.G + r % a.G) * a.o_h + d] =
-          __float2bfloat16(len - a.Sq + 1 + r / a.G <= 0 ? 0.f : num / den);
-    } else {
-      const long long row = (((long long)split * a.B + b) * a.Hk + h) * a.R + r;
-      a.part_o[row * HD + d] = num;
-      if (d == 0) {
-        a.part_ml[row * 2] = M;
-        a.part_ml[row * 2 + 1] = den;
+      for (int nt = 0; nt < NT; nt++) lim[nt][0] = sees[nt][0] - key0, lim[nt][1] = sees[nt][1] - key0;
+      const bool masked = key0 + KT > len - a.Sq + 1;
+      const int valid = len - key0;
+      auto kt = [&](int r, int piece) { return lds128(kb + r * 128 + ((piece ^ (r & 7)) << 4)); };
+      auto vt = [&](int r, int piece) {
+        uint4 v = lds128(vb + r * 128 + ((piece ^ (r & 7)) << 4));
+        // e4m3 bytes past the length may be NaN codes, which a weight of 0 would not cancel
+        if (FMT == CACHE_E4M3 && r >= valid) v = make_uint4(0, 0, 0, 0);
+        return v;
+      };
+      attend_tile<NT, FMT>(st, qf, kt, vt, sc.k, sc.v, lim, masked, lane);
+      __syncwarp();  // every lane has read the stage
+      if (i + STAGES < n) {
+        if (lane == 0) fetch(s);
+        ahead.next(a);
       }
     }
+    if (++s == STAGES) {
+      s = 0;
+      ph ^= 1;
+    }
+    if (i + 1 == n || then.t == 0) {  // the unit, or this run's part of it, ends here
+      // u + run grows from one piece of the sequence to the next, so it numbers the partial results
+      const long long slot = (long long)at.b * a.Hk * a.n_group + at.hg + run;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float l = st.l[nt][e];
+          l += __shfl_xor_sync(0xffffffffu, l, 4);
+          l += __shfl_xor_sync(0xffffffffu, l, 8);
+          l += __shfl_xor_sync(0xffffffffu, l, 16);
+          if (qf.row[nt][e] >= a.R) continue;
+          const long long row = slot * (8 * NT) + nt * 8 + 2 * c + e;
+          if (g == 0) __stcg(a.part_ml + row, make_float2(ok ? st.m[nt][e] : -INFINITY, l));
+          float4* const dst = reinterpret_cast<float4*>(a.part_o + row * HD + 16 * g);
+#pragma unroll
+          for (int j = 0; j < 8; j += 2)
+            __stcg(dst + j / 2, make_float4(st.o[j][nt][e], st.o[j][nt][2 + e], st.o[j + 1][nt][e], st.o[j + 1][nt][2 + e]));
+        }
+      }
+      if (i + 1 < n) {
+        at = then;
+        enter();
+      }
+    }
+    at = then;
+    sc = sc_next;
+  }
+  if (!ok) {  // let this warp's copies in flight land before the shared memory goes away
+    const long long t0 = clock64();
+    while ((unsigned long long)(clock64() - t0) < FT_WAIT_LIMIT_CYCLES / 4) __nanosleep(1000);
   }
 }
 
-__global__ void __launch_bounds__(HD) cache_combine_kernel(DecArgs a) {
-  const long long row = blockIdx.x;  // (b * Hk + h) * R + r
-  const int r = (int)(row % a.R), h = (int)(row / a.R % a.Hk), b = (int)(row / a.R / a.Hk), d = threadIdx.x;
+// Rows of the output: each row's partial results in run order, `merge_per_row` warps a row (each a
+// contiguous part of them), four dims a lane.
+template <int NT>
+__global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(DecArgs a) {
+  __shared__ float4 so[MERGE_WARPS][32];
+  __shared__ float2 sml[MERGE_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = a.merge_per_row, rows_here = MERGE_WARPS / per, part = warp % per;
   const long long rows = (long long)a.B * a.Hk * a.R;
-  float M = -INFINITY;
-  for (int s = 0; s < a.n_split; s++) M = max_nan(M, a.part_ml[(s * rows + row) * 2]);
-  float num = 0.f, den = 0.f;
-  for (int s = 0; s < a.n_split; s++) {
-    const float m = a.part_ml[(s * rows + row) * 2];
-    if (m == -INFINITY) continue;
-    const float f = ex2f(m - M);
-    den += f * a.part_ml[(s * rows + row) * 2 + 1];
-    num += f * a.part_o[(s * rows + row) * HD + d];
+  const long long row = (long long)blockIdx.x * rows_here + warp / per;  // (b * Hk + h) * R + r
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float M = -INFINITY, L = 0.f;
+  int r = 0, h = 0, b = 0, len = 0;
+  if (row < rows) {
+    r = (int)(row % a.R);
+    h = (int)(row / a.R % a.Hk);
+    b = (int)(row / a.R / a.Hk);
+    len = seq_len(a, b);
+    const int n = (len + KT - 1) / KT, hg = h * a.n_group + r / (8 * NT);
+    const Runs runs(tiles_before(a, a.B, lane) * a.Hk * a.n_group, a.runs);
+    const long long f = tiles_before(a, b, lane) * a.Hk * a.n_group + (long long)hg * n;
+    pdl_wait();
+    if (n > 0) {
+      const int r0 = runs.owner(f), r1 = runs.owner(f + n - 1) + 1, cnt = r1 - r0;
+      const int lo = r0 + cnt * part / per, hi = r0 + cnt * (part + 1) / per;
+      const long long base = ((long long)b * a.Hk * a.n_group + hg) * (8 * NT) + r % (8 * NT);
+      for (int i0 = lo; i0 < hi; i0 += 32) {  // references of 32 partials at once, then their rows
+        const float2 ml = i0 + lane < hi ? __ldcg(a.part_ml + base + (long long)(i0 + lane) * (8 * NT)) : make_float2(-INFINITY, 0.f);
+        float top = ml.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float m_new = max_nan(M, top), ref = m_new == -INFINITY ? 0.f : m_new;
+        const float al = M == -INFINITY ? 0.f : ex2f(M - ref), w = ml.x == -INFINITY ? 0.f : ex2f(ml.x - ref);
+        float l = w * ml.y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        M = m_new;
+        L = L * al + l;
+        acc.x *= al;
+        acc.y *= al;
+        acc.z *= al;
+        acc.w *= al;
+        const int m = min(32, hi - i0);
+#pragma unroll 4
+        for (int i = 0; i < m; i++) {
+          const float wi = __shfl_sync(0xffffffffu, w, i);
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + (base + (long long)(i0 + i) * (8 * NT)) * HD) + lane);
+          acc.x = fmaf(wi, v.x, acc.x);
+          acc.y = fmaf(wi, v.y, acc.y);
+          acc.z = fmaf(wi, v.z, acc.z);
+          acc.w = fmaf(wi, v.w, acc.w);
+        }
+      }
+    }
   }
-  a.o[b * a.o_b + (long long)(r / a.G) * a.o_tok + (long long)(h * a.G + r % a.G) * a.o_h + d] =
-      __float2bfloat16(seq_len(a, b) - a.Sq + 1 + r / a.G <= 0 ? 0.f : num / den);
+  if (per > 1) {
+    so[warp][lane] = acc;
+    if (lane == 0) sml[warp] = make_float2(M, L);
+    __syncthreads();
+    if (part != 0) return;
+    float top = M;
+    for (int i = 1; i < per; i++) top = max_nan(top, sml[warp + i].x);
+    const float ref = top == -INFINITY ? 0.f : top;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    L = 0.f;
+    for (int i = 0; i < per; i++) {
+      const float w = sml[warp + i].x == -INFINITY ? 0.f : ex2f(sml[warp + i].x - ref);
+      const float4 v = so[warp + i][lane];
+      acc.x = fmaf(w, v.x, acc.x);
+      acc.y = fmaf(w, v.y, acc.y);
+      acc.z = fmaf(w, v.z, acc.z);
+      acc.w = fmaf(w, v.w, acc.w);
+      L += w * sml[warp + i].y;
+    }
+  }
+  if (row >= rows) return;
+  const float inv = 1.f / L;
+  uint2 out = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  if (len - a.Sq + 1 + r / a.G <= 0) out = make_uint2(0, 0);  // the row sees no key
+  *reinterpret_cast<uint2*>(a.o + b * a.o_b + (long long)(r / a.G) * a.o_tok + (long long)(h * a.G + r % a.G) * a.o_h + 4 * lane) = out;
 }
 
 int rows_of(const CacheDecodeProblem& p) { return p.Sq * (p.Hq / p.Hk); }
 int col_tiles(const CacheDecodeProblem& p) { return rows_of(p) > 8 ? 2 : 1; }
 int groups_of(const CacheDecodeProblem& p) { return (rows_of(p) + 8 * col_tiles(p) - 1) / (8 * col_tiles(p)); }
 
-// about four CTAs an SM, each with at least two tiles a warp
-int splits_of(const CacheDecodeProblem& p) {
-  const long long base = (long long)p.B * p.Hk * groups_of(p);
-  const int tiles = (p.max_len + KT - 1) / KT;
-  const long long n = (4LL * p.num_sms + base - 1) / base;
-  return (int)max(1LL, min(n, (long long)(tiles / (2 * NWARP))));
+long long units_of(const CacheDecodeProblem& p) { return (long long)p.B * p.Hk * groups_of(p); }
+int runs_of(const CacheDecodeProblem& p) { return p.num_sms * NWARP; }
+long long partials_of(const CacheDecodeProblem& p) { return (units_of(p) + runs_of(p)) * 8 * col_tiles(p); }
+
+// One map of a cache side: [128 bytes][heads][tokens][sequences]. A broadcast dimension (stride 0)
+// is mapped with one entry.
+bool side_map(CUtensorMap* m, const CacheSide& s, const CacheDecodeProblem& p, int& one_b, int& one_h) {
+  one_b = p.B == 1 || s.c_b == 0;
+  one_h = p.Hk == 1 || s.c_h == 0;
+  return make_tmap_4d_u8(m, s.codes, HD, one_h ? 1 : p.Hk, p.L, one_b ? 1 : p.B, one_h ? HD : s.c_h,
+                         p.L == 1 ? HD : s.c_tok, one_b ? HD : s.c_b, HD, 1, KT, 1);
+}
+
+template <int NT, int FMT>
+cudaError_t launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecArgs& a, int sms, cudaStream_t stream) {
+  const int smem = (int)sizeof(DecSmem) + 1024;
+  static bool attr = false;
+  if (!attr) {
+    const cudaError_t e = cudaFuncSetAttribute(cache_decode_kernel<NT, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    attr = true;
+  }
+  cache_decode_kernel<NT, FMT><<<sms, 32 * NWARP, smem, stream>>>(tk, tv, a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // the merge may start while the first kernel's last CTAs run; it waits for them before it reads
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  const long long rows = (long long)a.B * a.Hk * a.R;
+  cfg.gridDim = dim3((unsigned)((rows * a.merge_per_row + MERGE_WARPS - 1) / MERGE_WARPS));
+  cfg.blockDim = dim3(32 * MERGE_WARPS);
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, cache_merge_kernel<NT>, a);
 }
 
 }  // namespace
 
-size_t cache_decode_scratch_floats(const CacheDecodeProblem& p) {
-  const int n = splits_of(p);
-  return n > 1 ? (size_t)n * p.B * p.Hk * rows_of(p) * (HD + 2) : 0;
-}
-
-int cache_decode_launches(const CacheDecodeProblem& p) { return splits_of(p) > 1 ? 2 : 1; }
+size_t cache_decode_scratch_floats(const CacheDecodeProblem& p) { return (size_t)partials_of(p) * (HD + 2); }
 
 cudaError_t cache_append(const CacheAppendProblem& p, cudaStream_t stream) {
   if (p.B <= 0 || p.S <= 0 || p.Hk <= 0) return cudaSuccess;
@@ -608,25 +849,23 @@ cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream) {
   a.len_all = p.len_all;
   a.max_len = p.max_len;
   a.scale_log2 = p.scale * 1.4426950408889634f;
-  a.n_split = splits_of(p);
+  a.runs = runs_of(p);
   const long long rows = (long long)p.B * p.Hk * a.R;
-  if (rows > 0x7fffffffLL || p.B > 65535 || (long long)p.Hk * a.n_group > 65535) return cudaErrorInvalidValue;
-  if (a.n_split > 1 && p.scratch == nullptr) return cudaErrorInvalidValue;
+  // units, runs and rows are numbered in 32 bits on the way
+  if (rows > 0x3fffffffLL || units_of(p) > 0x3fffffffLL || p.B > (1 << 24)) return cudaErrorInvalidValue;
+  if (p.scratch == nullptr) return cudaErrorInvalidValue;
   a.part_o = p.scratch;
-  a.part_ml = p.scratch ? p.scratch + (size_t)a.n_split * rows * HD : nullptr;
-  const dim3 grid(a.n_split, p.Hk * a.n_group, p.B);
+  a.part_ml = reinterpret_cast<float2*>(p.scratch + (size_t)partials_of(p) * HD);
+  // a row has about runs / units partials; warps that share it take a few each
+  const long long expect = a.runs / units_of(p);
+  a.merge_per_row = expect >= 64 ? 8 : expect >= 16 ? 4 : expect >= 8 ? 2 : 1;
+  CUtensorMap tk, tv;
+  if (p.L > 0 && (!side_map(&tk, p.side[0], p, a.one_b[0], a.one_h[0]) || !side_map(&tv, p.side[1], p, a.one_b[1], a.one_h[1])))
+    return cudaErrorInvalidValue;
   const bool i8 = p.format == CACHE_INT8;
-  if (col_tiles(p) == 1) {
-    if (i8) cache_decode_kernel<1, CACHE_INT8><<<grid, 32 * NWARP, 0, stream>>>(a);
-    else cache_decode_kernel<1, CACHE_E4M3><<<grid, 32 * NWARP, 0, stream>>>(a);
-  } else {
-    if (i8) cache_decode_kernel<2, CACHE_INT8><<<grid, 32 * NWARP, 0, stream>>>(a);
-    else cache_decode_kernel<2, CACHE_E4M3><<<grid, 32 * NWARP, 0, stream>>>(a);
-  }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || a.n_split == 1) return e;
-  cache_combine_kernel<<<(unsigned)rows, HD, 0, stream>>>(a);
-  return cudaGetLastError();
+  if (col_tiles(p) == 1)
+    return i8 ? launch_decode<1, CACHE_INT8>(tk, tv, a, p.num_sms, stream) : launch_decode<1, CACHE_E4M3>(tk, tv, a, p.num_sms, stream);
+  return i8 ? launch_decode<2, CACHE_INT8>(tk, tv, a, p.num_sms, stream) : launch_decode<2, CACHE_E4M3>(tk, tv, a, p.num_sms, stream);
 }
 
 }  // namespace ft

@@ -27,7 +27,7 @@ struct MoeDecodeProblem {
   void* workspace = nullptr;              // moe_decode_workspace(p) bytes, 256-byte aligned
 };
 size_t moe_decode_workspace(const MoeDecodeProblem& p);
-int moe_decode_launches(const MoeDecodeProblem& p);
+// four kernels
 cudaError_t moe_decode(const MoeDecodeProblem& p, cudaStream_t stream);
 int moe_decode_device_error(bool reset);
 

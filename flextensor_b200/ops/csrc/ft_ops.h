@@ -53,6 +53,10 @@ bool make_tmap_3d_bf16(CUtensorMap* map, const void* base, uint64_t inner, uint6
 bool make_tmap_4d_bf16(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t d3,
                        uint64_t s1, uint64_t s2, uint64_t s3, int b0, int b1, int b2, int b3);
 
+// The same over bytes: strides in bytes (multiples of 16), 128-byte swizzle when b0 == 128.
+bool make_tmap_4d_u8(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t d3,
+                     uint64_t s1, uint64_t s2, uint64_t s3, int b0, int b1, int b2, int b3);
+
 // Decode attention (decode_sm100.cu): q [B, Hq, 128] (one query per sequence) over a KV cache
 // [B, L, Hk, 128] (token / batch strides in elements), keys [0, len_b) of sequence b.
 struct DecodeProblem {

@@ -559,8 +559,6 @@ cudaError_t launch_all(const MoeDecodeProblem& p, const Args& a, cudaStream_t st
 
 size_t moe_decode_workspace(const MoeDecodeProblem& p) { return layout_of(p).bytes; }
 
-int moe_decode_launches(const MoeDecodeProblem&) { return 4; }
-
 cudaError_t moe_decode(const MoeDecodeProblem& p, cudaStream_t stream) {
   if (p.T <= 0) return cudaSuccess;
   if (p.T > MAX_T || p.E < 1 || p.E > MAX_E || p.topk < 1 || p.topk > MAX_K || p.topk > p.E || p.D < 8 || p.F < 8 ||
