@@ -21,12 +21,17 @@
 //      interleaved with PRMT into the (key, key+1) pairs the MMA wants.
 // P goes from the accumulator layout to the B operand with one 8x8 transpose per 8 keys.
 //
-// Work. All (sequence, KV head, row group) units form one sequence of 32-key tiles, divided into
-// equal contiguous runs, one per warp (8 warps an SM), so ragged batches and few long sequences load
-// every SM alike. A warp streams its run by itself through its own three 8 KB stages (TMA, 128-byte
-// swizzle; the warp's own program order says when a stage is free, so there is no producer and no
-// barrier between warps) and writes fp32 partial results at unit ends; a second kernel, launched
-// so that its start overlaps the first one's end, merges the partials of each row in run order.
+// Work. The eight warps of a CTA (one CTA an SM) take tiles of as many heads side by side as divide
+// the heads (8, 4, 2 or 1), and consecutive tiles of a head where that leaves warps over. The units
+// of 32 keys of those heads, in the order sequence, heads, keys, are divided into equal contiguous
+// runs, one per CTA, so ragged batches and few long sequences load every SM alike. Heads side by side
+// matter because one token's heads are neighbours in memory: with a run per warp, each in its own
+// head, the same copies took 34.8 us instead of 26.5 (32 x 2304 tokens, 8 heads) and 54 us instead of
+// 42 (131071 tokens) without any arithmetic. A warp streams its tiles by itself through three 8 KB
+// slots that hold 64 keys and their values in turn (TMA, 128-byte swizzle; the warp's own program
+// order says when a slot is free, so there is no producer and no barrier between warps) and writes
+// fp32 partial results where its head or its run end; a second kernel, launched so that its start
+// overlaps the first one's end, merges the partials of each row in a fixed order.
 //
 // Scales: a score is (q . codes) * ks, and the weight of a value's codes is p * vs. The running
 // reference m is the maximum of score + log2(vs), so p * vs <= 1 whatever the scales are and f16
@@ -37,6 +42,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "ft_cache.h"
 #include "ft_ops.h"
@@ -49,6 +56,27 @@ FT_DEFINE_ERROR_READER(cache_device_error)
 namespace {
 
 constexpr int HD = 128;  // head dim
+
+// Every kernel here is launched so that it may start while the kernel before it in the stream ends
+// (programmatic serialization): it waits for that kernel's results before it reads any memory. No load
+// takes the non-coherent path, which that wait says nothing about.
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... P, class... A>
+cudaError_t launch_overlapped(void (*kernel)(P...), unsigned grid, int threads, int smem, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
 
 // ------------------------------------------------------------------------------------ writing
 struct AppendArgs {
@@ -106,6 +134,8 @@ __global__ void __launch_bounds__(BLOCK <= 64 ? 128 : 256) cache_append_kernel(A
   constexpr int ROWS = THREADS / 16;  // token rows per pass: 16 lanes hold a row's 128 values
   constexpr int ITERS = BLOCK / ROWS;
   __shared__ uint32_t warp_max[THREADS / 32];
+  pdl_wait();
+  pdl_launch();
   long long id = blockIdx.x;
   const int h = (int)(id % a.Hk);
   id /= a.Hk;
@@ -132,7 +162,7 @@ __global__ void __launch_bounds__(BLOCK <= 64 ? 128 : 256) cache_append_kernel(A
   for (int i = 0; i < ITERS; i++) {
     const int t = j * BLOCK + i * ROWS + row0;
     v[i] = make_uint4(0, 0, 0, 0);
-    if (t >= t0 && t < t1) v[i] = __ldg(reinterpret_cast<const uint4*>(x + (long long)(t - p) * a.x_tok[kv]));
+    if (t >= t0 && t < t1) v[i] = *reinterpret_cast<const uint4*>(x + (long long)(t - p) * a.x_tok[kv]);
   }
 #pragma unroll
   for (int i = 0; i < ITERS; i++) {
@@ -180,23 +210,25 @@ cudaError_t launch_append(const AppendArgs& a, int format, cudaStream_t stream) 
   const long long grid = (long long)a.B * 2 * a.n_rel * a.Hk;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
   const int threads = BLOCK <= 64 ? 128 : 256;
-  if (format == CACHE_INT8) cache_append_kernel<BLOCK, CACHE_INT8><<<(unsigned)grid, threads, 0, stream>>>(a);
-  else cache_append_kernel<BLOCK, CACHE_E4M3><<<(unsigned)grid, threads, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_overlapped(format == CACHE_INT8 ? cache_append_kernel<BLOCK, CACHE_INT8> : cache_append_kernel<BLOCK, CACHE_E4M3>,
+                           (unsigned)grid, threads, 0, stream, a);
 }
 
 // ------------------------------------------------------------------------------------ attention
-constexpr int KT = 32;       // keys of a tile
-constexpr int NWARP = 8;
-constexpr int STAGES = 3;    // per warp
-constexpr int SIDE_BYTES = KT * HD;
-constexpr int STAGE_BYTES = 2 * SIDE_BYTES;  // keys, values
-constexpr int MERGE_WARPS = 8;
+constexpr int UNIT = 32;     // keys: what runs are made of
+constexpr int WARPS = 8;
+constexpr int SLOTS = 3;     // per warp, keys and values in turn
+// Units of a tile: two column tiles leave registers for one
+constexpr int units_of_tile(int column_tiles) { return column_tiles == 1 ? 2 : 1; }
+constexpr int UNIT_BYTES = UNIT * HD;
+constexpr int MERGE_WARPS = 16;  // at most
 
 struct DecArgs {
   int B, Sq, Hq, Hk, L, G, R, n_group;  // R = Sq * G query rows of a KV head in n_group groups of 8 * NT
   int block_shift;
-  int runs;                             // warps that may take a run
+  int heads, keys;                      // (head, group) units and key tiles side by side in a CTA: heads * keys = WARPS
+  int per;                              // Hk * n_group / heads: steps of heads in a sequence
+  int runs;                             // CTAs
   const __nv_bfloat16* q;
   long long q_b, q_tok, q_h;
   __nv_bfloat16* o;
@@ -206,8 +238,8 @@ struct DecArgs {
   const int* kv_len;
   int len_all, max_len;
   float scale_log2;                     // softmax scale * log2(e)
-  float* part_o;                        // [units + runs][8 * NT][128]
-  float2* part_ml;                      // [units + runs][8 * NT] reference and sum
+  float* part_o;                        // [steps of heads + runs][WARPS][8 * NT][128]
+  float2* part_ml;                      // [steps of heads + runs][WARPS][8 * NT] reference and sum
   int merge_per_row;                    // warps that share a row of the merge
 };
 
@@ -322,25 +354,39 @@ struct RowState {
   float m[NT][2], l[NT][2];
 };
 
-// One tile of KT keys: `kt`/`vt` give 16-byte pieces (row, piece) of the tile's codes, `lim` the
-// number of keys of the tile that each column sees (KT or more: all).
-template <int NT, int FMT, class KLoad, class VLoad>
+// The scales of a tile's 16-key groups: keys' scale, values' scale, its log2 (the reference of the
+// weights) and its inverse. A group whose scale is not an ordinary number gets a weight of its own.
+template <int MT>
+struct TileScales {
+  float k[MT], v[MT];
+};
+
+// One tile of 16 * MT keys: `kt`/`vt` give 16-byte pieces (row, piece) of the tile's codes, `lim` the
+// number of keys of the tile that each column sees (16 * MT or more: all). `keys_read` is called when
+// the keys have been read, `values_here` before the values are.
+template <int NT, int MT, int FMT, class KLoad, class VLoad, class KDone, class VReady>
 __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT>& qf, KLoad kt, VLoad vt,
-                                            const float (&ks)[KT / 16], const float (&vs)[KT / 16],
-                                            const int (&lim)[NT][2], bool masked, int lane) {
+                                            const TileScales<MT>& sc, const int (&lim)[NT][2], bool masked, int lane,
+                                            KDone keys_read, VReady values_here) {
   const int g = lane >> 2, c = lane & 3;
-  constexpr int MT = KT / 16;
   float s[MT][NT][4];
 #pragma unroll
-  for (int mt = 0; mt < MT; mt++) {
+  for (int mt = 0; mt < MT; mt++)
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
 #pragma unroll
-    for (int hh = 0; hh < 2; hh++) {
-      const uint4 x = kt(mt * 16 + g, 2 * c + hh), y = kt(mt * 16 + g + 8, 2 * c + hh);
-      const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+  for (int hh = 0; hh < 2; hh++) {
+    uint4 x[MT], y[MT];
 #pragma unroll
-      for (int w = 0; w < 4; w++) {
+    for (int mt = 0; mt < MT; mt++) {
+      x[mt] = kt(mt * 16 + g, 2 * c + hh);
+      y[mt] = kt(mt * 16 + g + 8, 2 * c + hh);
+    }
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++) {  // MT independent chains
+        const uint32_t xw[4] = {x[mt].x, x[mt].y, x[mt].z, x[mt].w}, yw[4] = {y[mt].x, y[mt].y, y[mt].z, y[mt].w};
         uint32_t a0, a1, a2, a3;
         decode4<FMT>(xw[w], a0, a2);
         decode4<FMT>(yw[w], a1, a3);
@@ -350,55 +396,79 @@ __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT
       }
     }
   }
-  float lv[MT];
+  keys_read();
+  float lv[MT], iv[MT];
+  bool odd = false;  // a value scale that is 0, tiny, huge or NaN
 #pragma unroll
-  for (int mt = 0; mt < MT; mt++) lv[mt] = lg2f(fmaxf(vs[mt], 0x1p-100f));
+  for (int mt = 0; mt < MT; mt++) {
+    odd |= !(sc.v[mt] >= 0x1p-100f && sc.v[mt] <= 0x1p100f);
+    const float v = fminf(fmaxf(sc.v[mt], 0x1p-100f), 0x1p100f);
+    lv[mt] = lg2f(v);
+    iv[mt] = __fdividef(1.f, v);
+  }
   uint32_t pb[MT][NT][2];
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
-    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        float z = s[mt][nt][e] * (ks[mt] * qf.fac[nt][e & 1]);
-        if (masked && mt * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1]) z = -INFINITY;
-        s[mt][nt][e] = z;
-        top[e & 1] = max_nan(top[e & 1], z + lv[mt]);
-      }
+      const float f0 = sc.k[mt] * qf.fac[nt][0], f1 = sc.k[mt] * qf.fac[nt][1];
+      s[mt][nt][0] *= f0;
+      s[mt][nt][1] *= f1;
+      s[mt][nt][2] *= f0;
+      s[mt][nt][3] *= f1;
     }
+    if (masked) {
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (mt * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1]) s[mt][nt][e] = -INFINITY;
+    }
+    float top[2];
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 4));
-      top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 8));
-      top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
-      const float m_new = max_nan(st.m[nt][i], top[i]);
-      const float ref = m_new == -INFINITY ? 0.f : m_new;
-      const float al = st.m[nt][i] == -INFINITY ? 0.f : ex2f(st.m[nt][i] - ref);
-      st.m[nt][i] = m_new;
-      st.l[nt][i] *= al;
+      top[i] = max_nan(s[0][nt][i], s[0][nt][2 + i]) + lv[0];
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        st.o[j][nt][i] *= al;
-        st.o[j][nt][2 + i] *= al;
-      }
-      top[i] = ref;
+      for (int mt = 1; mt < MT; mt++) top[i] = max_nan(top[i], max_nan(s[mt][nt][i], s[mt][nt][2 + i]) + lv[mt]);
     }
+    // the reference moves only when a weight would pass 2^8 (f16 holds 2^15), so the accumulators are
+    // seldom rescaled; all lanes of a column take the same one
+    const bool grow = !(top[0] <= st.m[nt][0] + 8.f) || !(top[1] <= st.m[nt][1] + 8.f);
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 4));
+        top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 8));
+        top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
+        const float m_new = max_nan(st.m[nt][i], top[i]);
+        const float al = st.m[nt][i] == -INFINITY ? 0.f : ex2f(st.m[nt][i] - m_new);
+        st.m[nt][i] = m_new;
+        st.l[nt][i] *= al;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          st.o[j][nt][i] *= al;
+          st.o[j][nt][2 + i] *= al;
+        }
+      }
+    }
+    const float ref[2] = {st.m[nt][0] == -INFINITY ? 0.f : st.m[nt][0], st.m[nt][1] == -INFINITY ? 0.f : st.m[nt][1]};
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) {
-      float w[4];
+      const float d0 = lv[mt] - ref[0], d1 = lv[mt] - ref[1];
+      float w[4] = {ex2f(s[mt][nt][0] + d0), ex2f(s[mt][nt][1] + d1), ex2f(s[mt][nt][2] + d0), ex2f(s[mt][nt][3] + d1)};
+      st.l[nt][0] = fmaf(w[0] + w[2], iv[mt], st.l[nt][0]);
+      st.l[nt][1] = fmaf(w[1] + w[3], iv[mt], st.l[nt][1]);
+      if (odd) {  // the weight is p * vs: 0 for a scale of 0, NaN for NaN, and 0 for what the column does not see
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float p = ex2f(s[mt][nt][e] - top[e & 1]);
-        st.l[nt][e & 1] += p;
-        // a key that the column does not see weighs exactly 0, whatever its block's scale
-        w[e] = masked && mt * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1] ? 0.f : p * vs[mt];
+        for (int e = 0; e < 4; e++)
+          w[e] = masked && mt * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1] ? 0.f : w[e] * iv[mt] * sc.v[mt];
       }
       __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
       pb[mt][nt][0] = transpose8x8(*reinterpret_cast<uint32_t*>(&h0));
       pb[mt][nt][1] = transpose8x8(*reinterpret_cast<uint32_t*>(&h1));
     }
   }
+  if (!values_here()) return;
 #pragma unroll
   for (int mt = 0; mt < MT; mt++) {
     const uint4 v0 = vt(mt * 16 + 2 * c, g), v1 = vt(mt * 16 + 2 * c + 1, g);
@@ -422,80 +492,89 @@ __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT
 }
 
 __device__ __forceinline__ int seq_len(const DecArgs& a, int b) {
-  return max(0, min(a.kv_len ? __ldg(a.kv_len + b) : a.len_all, a.max_len));
+  return max(0, min(a.kv_len ? a.kv_len[b] : a.len_all, a.max_len));
 }
-__device__ __forceinline__ int seq_tiles(const DecArgs& a, int b) { return (seq_len(a, b) + KT - 1) / KT; }
+__device__ __forceinline__ int seq_units(const DecArgs& a, int b) { return (seq_len(a, b) + UNIT - 1) / UNIT; }
 
-// sum of the tiles of sequences [0, end) of one KV head and row group, by a whole warp
-__device__ __forceinline__ long long tiles_before(const DecArgs& a, int end, int lane) {
-  if (a.kv_len == nullptr) return (long long)end * seq_tiles(a, 0);
-  long long sum = 0;
-  for (int b = lane; b < end; b += 32) sum += seq_tiles(a, b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
+// sum of the units of sequences [0, end) over all steps of heads, by a whole warp
+__device__ __forceinline__ int units_before(const DecArgs& a, int end, int lane) {
+  if (a.kv_len == nullptr) return end * seq_units(a, 0) * a.per;
+  int sum = 0;
+  for (int b = lane; b < end; b += 32) sum += seq_units(a, b);
+  return __reduce_add_sync(0xffffffffu, sum) * a.per;
 }
 
-// The sequence of tiles and its division into runs.
+// The sequence of units (fewer than 2^30, the host checks) and its division into runs, the first
+// `rem` of them one unit longer.
 struct Runs {
-  long long total;
-  int n;
-  __device__ __forceinline__ Runs(long long t, int most) : total(t), n((int)min((long long)most, t)) {}
-  __device__ __forceinline__ long long begin(int r) const { return total * r / n; }
-  __device__ __forceinline__ int owner(long long i) const { return (int)(((i + 1) * n - 1) / total); }
-};
-
-// A place in the sequence of tiles.
-struct Cursor {
-  int b, hg, t, n;  // sequence, head * n_group + group, tile of the unit, tiles of a unit of this sequence
-  __device__ __forceinline__ void next(const DecArgs& a) {
-    if (++t < n) return;
-    t = 0;
-    if (++hg < a.Hk * a.n_group) return;
-    hg = 0;
-    do {
-      if (++b >= a.B) return;
-      n = seq_tiles(a, b);
-    } while (n == 0);
+  int n, base, rem;
+  __device__ __forceinline__ Runs(int total, int most) : n(min(most, total)) {
+    base = n ? total / n : 0;
+    rem = total - base * n;
+  }
+  __device__ __forceinline__ int begin(int r) const { return r * base + min(r, rem); }
+  __device__ __forceinline__ int owner(int i) const {
+    const int longer = rem * (base + 1);
+    return i < longer ? i / (base + 1) : rem + (i - longer) / base;
   }
 };
 
-// the place of tile i, by a whole warp
-__device__ __forceinline__ Cursor locate(const DecArgs& a, long long i, int lane) {
+// A warp's place in its CTA's run: a tile of units [t, min(t + units of a tile, end)) of a piece, the
+// run's part of one step of heads of one sequence.
+struct Cursor {
+  int b, j, t, end, left;  // sequence, step of heads, first unit, end of the piece, units of the run after the piece
+
+  // the tile `step` units further on, `start` units into a piece where that leaves this one; false at the run's end
+  __device__ __forceinline__ bool next(const DecArgs& a, int step, int start) {
+    t += step;
+    while (t >= end) {
+      if (left == 0) return false;
+      int n = 0;
+      if (++j == a.per) j = 0, b++;
+      while ((n = seq_units(a, b)) == 0) b++;  // units are left, so a sequence with some follows
+      end = min(n, left);
+      left -= end;
+      t = start;
+    }
+    return true;
+  }
+};
+
+// the place of unit i, the first of a run of `count` units, by a whole warp
+__device__ __forceinline__ Cursor locate(const DecArgs& a, int i, int count, int lane) {
   Cursor c;
-  const int per = a.Hk * a.n_group;
+  int n;
   if (a.kv_len == nullptr) {
-    c.n = seq_tiles(a, 0);
-    c.b = (int)(i / ((long long)c.n * per));
-    i -= (long long)c.b * c.n * per;
+    n = seq_units(a, 0);
+    c.b = i / (n * a.per);
+    i -= c.b * n * a.per;
   } else {
-    long long before = 0;
+    int before = 0;
     for (int b0 = 0;; b0 += 32) {  // i lies before the total, so some sequence holds it
-      const int n = b0 + lane < a.B ? seq_tiles(a, b0 + lane) : 0;
-      long long end = n;
+      const int mine = b0 + lane < a.B ? seq_units(a, b0 + lane) : 0;
+      int end = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, end, o);
+        const int up = __shfl_up_sync(0xffffffffu, end, o);
         if (lane >= o) end += up;
       }
-      const unsigned int hit = __ballot_sync(0xffffffffu, (before + end) * per > i);
+      const unsigned int hit = __ballot_sync(0xffffffffu, (before + end) * a.per > i);
       if (hit || b0 + 32 >= a.B) {
         const int at = hit ? __ffs(hit) - 1 : 31;
         c.b = b0 + at;
-        c.n = __shfl_sync(0xffffffffu, n, at);
-        i -= (before + __shfl_sync(0xffffffffu, end - n, at)) * per;
+        n = __shfl_sync(0xffffffffu, mine, at);
+        i -= (before + __shfl_sync(0xffffffffu, end - mine, at)) * a.per;
         break;
       }
       before += __shfl_sync(0xffffffffu, end, 31);
     }
   }
-  c.hg = (int)(i / c.n);
-  c.t = (int)(i % c.n);
+  c.j = i / n;
+  c.t = i - c.j * n;
+  c.end = min(n, c.t + count);
+  c.left = count - (c.end - c.t);
   return c;
 }
-
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z, int w) {
   asm volatile(
@@ -524,64 +603,87 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   return v;
 }
 
+template <int NT>
 struct DecSmem {
-  uint8_t stage[NWARP][STAGES][STAGE_BYTES];
-  uint64_t full[NWARP][STAGES];
+  uint8_t slot[WARPS][SLOTS][units_of_tile(NT) * UNIT_BYTES];
+  uint64_t full[WARPS][SLOTS];
 };
-
-struct TileScales {
-  float k[KT / 16], v[KT / 16];
-};
-
-// 16 keys never straddle a block; a tile's tail past the length takes the last block's scale
-__device__ __forceinline__ TileScales load_scales(const DecArgs& a, const Cursor& c) {
-  TileScales s;
-  const int h = c.hg / a.n_group, last = seq_len(a, c.b) - 1;
-#pragma unroll
-  for (int i = 0; i < KT / 16; i++) {
-    const long long blk = min(c.t * KT + 16 * i, last) >> a.block_shift;
-    s.k[i] = __ldg(a.k.scale + c.b * a.k.s_b + blk * a.k.s_blk + h * a.k.s_h);
-    s.v[i] = __ldg(a.v.scale + c.b * a.v.s_b + blk * a.v.s_blk + h * a.v.s_h);
-  }
-  return s;
-}
 
 template <int NT, int FMT>
-__global__ void __launch_bounds__(32 * NWARP, 1)
-    cache_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, DecArgs a) {
+__global__ void __launch_bounds__(32 * WARPS, 1)
+    cache_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                        const __grid_constant__ DecArgs a) {
+  constexpr int UT = units_of_tile(NT), MT = UT * UNIT / 16;
   extern __shared__ uint8_t smem_raw[];
-  DecSmem& sm = *reinterpret_cast<DecSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  DecSmem<NT>& sm = *reinterpret_cast<DecSmem<NT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  pdl_launch();
-  const Runs runs(tiles_before(a, a.B, lane) * a.Hk * a.n_group, a.runs);
-  const int run = warp * gridDim.x + blockIdx.x;  // neighbouring runs on different SMs: few runs spread out
-  if (run >= runs.n) return;
-  const long long first = runs.begin(run);
-  const int n = (int)(runs.begin(run + 1) - first);
   uint64_t* const full = sm.full[warp];
   if (lane == 0) {
-    for (int s = 0; s < STAGES; s++) mbar_init(&full[s], 1);
+    for (int s = 0; s < SLOTS; s++) mbar_init(&full[s], 1);
     fence_barrier_init();
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
   }
   __syncwarp();
-  Cursor at = locate(a, first, lane), ahead = at;
-  auto fetch = [&](int s) {  // one lane: the tile at `ahead` into stage s
-    const int h = ahead.hg / a.n_group, key0 = ahead.t * KT;
-    uint8_t* const dst = sm.stage[warp][s];
-    mbar_arrive_expect_tx(&full[s], STAGE_BYTES);
-    tma_load_4d(dst, &tm_k, &full[s], 0, a.one_h[0] ? 0 : h, key0, a.one_b[0] ? 0 : ahead.b);
-    tma_load_4d(dst + SIDE_BYTES, &tm_v, &full[s], 0, a.one_h[1] ? 0 : h, key0, a.one_b[1] ? 0 : ahead.b);
+  pdl_wait();
+  pdl_launch();
+  const Runs runs(units_before(a, a.B, lane), a.runs);
+  const int run = blockIdx.x;
+  if (run >= runs.n) return;
+  const int first = runs.begin(run), count = runs.begin(run + 1) - first;
+  const int my_head = warp % a.heads, start = warp / a.heads * UT, step = a.keys * UT;
+  Cursor at = locate(a, first, count, lane);
+  if (!at.next(a, start, start)) return;  // a run too short for this warp
+  Cursor ahead = at;
+  auto fetch = [&](int s, bool values) {  // keys or values of the tile at `ahead` into slot s
+    if (lane == 0) {
+      const int hg = ahead.j * a.heads + my_head, h = a.n_group == 1 ? hg : hg / a.n_group;
+      const int z = a.one_h[values] ? 0 : h, w = a.one_b[values] ? 0 : ahead.b;
+      const CUtensorMap* const map = values ? &tm_v : &tm_k;
+      uint8_t* const dst = sm.slot[warp][s];
+      const bool two = UT == 2 && ahead.t + 1 < ahead.end;
+      mbar_arrive_expect_tx(&full[s], two ? 2 * UNIT_BYTES : UNIT_BYTES);
+      tma_load_4d(dst, map, &full[s], 0, z, ahead.t * UNIT, w);
+      if (two) tma_load_4d(dst + UNIT_BYTES, map, &full[s], 0, z, (ahead.t + 1) * UNIT, w);
+    }
   };
-  for (int s = 0; s < STAGES && s < n; s++) {
-    if (lane == 0) fetch(s);
-    ahead.next(a);
-  }
+  fetch(0, false);
+  fetch(1, true);
+  bool more = ahead.next(a, step, start);  // whether `ahead` is a tile after `at`
+  if (more) fetch(2, false);
   QueryFrag<NT> qf;
   RowState<NT> st;
   int sees[NT][2], len = 0;
-  auto enter = [&]() {  // a new unit: its queries, empty accumulators
+  const float *ksp = nullptr, *vsp = nullptr;  // the head's scales
+  TileScales<MT> sc;
+  // 16 keys never straddle a block, and a tile of a whole block or less takes one scale; what lies
+  // past the length takes the last block's
+  auto scales = [&](int t) {
+    if (16 * MT <= 1 << a.block_shift) {
+      const int blk = (t * UNIT) >> a.block_shift, blk2 = min(t * UNIT + 16 * MT - 1, len - 1) >> a.block_shift;
+      const float k0 = ksp[(long long)blk * a.k.s_blk], v0 = vsp[(long long)blk * a.v.s_blk];
+      const float k1 = ksp[(long long)blk2 * a.k.s_blk], v1 = vsp[(long long)blk2 * a.v.s_blk];
+#pragma unroll
+      for (int i = 0; i < MT; i++) {  // a tile that starts at an odd unit may lie in two blocks, half in each
+        sc.k[i] = i < MT / 2 ? k0 : k1;
+        sc.v[i] = i < MT / 2 ? v0 : v1;
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+      const int blk = min(t * UNIT + 16 * i, len - 1) >> a.block_shift;
+      sc.k[i] = ksp[(long long)blk * a.k.s_blk];
+      sc.v[i] = vsp[(long long)blk * a.v.s_blk];
+    }
+  };
+  auto enter = [&]() {  // a new head: its queries, empty accumulators
+    const int hg = at.j * a.heads + my_head, h = hg / a.n_group;
     len = seq_len(a, at.b);
-    load_queries<NT>(qf, a, at.b, at.hg / a.n_group, at.hg % a.n_group * 8 * NT, lane);
+    ksp = a.k.scale + at.b * a.k.s_b + h * a.k.s_h;
+    vsp = a.v.scale + at.b * a.v.s_b + h * a.v.s_h;
+    scales(at.t);
+    load_queries<NT>(qf, a, at.b, h, (hg - h * a.n_group) * 8 * NT, lane);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -595,23 +697,31 @@ __global__ void __launch_bounds__(32 * NWARP, 1)
     }
   };
   enter();
-  TileScales sc = load_scales(a, at);
   bool ok = true;
-  int s = 0;
-  uint32_t ph = 0;
-  for (int i = 0; i < n; i++) {
-    Cursor then = at;
-    then.next(a);
-    const TileScales sc_next = i + 1 < n ? load_scales(a, then) : sc;
+  int s = 0;        // slot of the next piece to read
+  uint32_t ph = 0;  // and its phase
+  auto turn = [&]() {
+    if (++s == SLOTS) {
+      s = 0;
+      ph ^= 1;
+    }
+  };
+  for (;;) {
+    const bool last = !more || ahead.j != at.j || ahead.b != at.b;  // tile of this head
+    const int key0 = at.t * UNIT, here = min((at.end - at.t) * UNIT, 16 * MT);  // keys of the tile that are this run's
     if (ok) ok = __all_sync(0xffffffffu, bounded_wait(&full[s], ph));
+    const int sk = s;
+    turn();
     if (ok) {
-      const int key0 = at.t * KT;
-      const uint32_t kb = smem_u32(sm.stage[warp][s]), vb = kb + SIDE_BYTES;
       int lim[NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) lim[nt][0] = sees[nt][0] - key0, lim[nt][1] = sees[nt][1] - key0;
-      const bool masked = key0 + KT > len - a.Sq + 1;
-      const int valid = len - key0;
+      for (int nt = 0; nt < NT; nt++) {
+        lim[nt][0] = min(sees[nt][0] - key0, here);
+        lim[nt][1] = min(sees[nt][1] - key0, here);
+      }
+      const bool masked = here < 16 * MT || key0 + 16 * MT > len - a.Sq + 1;
+      const int valid = min(len - key0, here);
+      const uint32_t kb = smem_u32(sm.slot[warp][sk]), vb = smem_u32(sm.slot[warp][s]);
       auto kt = [&](int r, int piece) { return lds128(kb + r * 128 + ((piece ^ (r & 7)) << 4)); };
       auto vt = [&](int r, int piece) {
         uint4 v = lds128(vb + r * 128 + ((piece ^ (r & 7)) << 4));
@@ -619,20 +729,19 @@ __global__ void __launch_bounds__(32 * NWARP, 1)
         if (FMT == CACHE_E4M3 && r >= valid) v = make_uint4(0, 0, 0, 0);
         return v;
       };
-      attend_tile<NT, FMT>(st, qf, kt, vt, sc.k, sc.v, lim, masked, lane);
-      __syncwarp();  // every lane has read the stage
-      if (i + STAGES < n) {
-        if (lane == 0) fetch(s);
-        ahead.next(a);
-      }
+      auto keys_read = [&]() {  // the slot takes the values of the next tile
+        __syncwarp();
+        if (more) fetch(sk, true);
+      };
+      auto values_here = [&]() { return ok = __all_sync(0xffffffffu, bounded_wait(&full[s], ph)); };
+      const TileScales<MT> now = sc;
+      if (!last) scales(ahead.t);  // in flight during the tile
+      attend_tile<NT, MT, FMT>(st, qf, kt, vt, now, lim, masked, lane, keys_read, values_here);
+      __syncwarp();
     }
-    if (++s == STAGES) {
-      s = 0;
-      ph ^= 1;
-    }
-    if (i + 1 == n || then.t == 0) {  // the unit, or this run's part of it, ends here
-      // u + run grows from one piece of the sequence to the next, so it numbers the partial results
-      const long long slot = (long long)at.b * a.Hk * a.n_group + at.hg + run;
+    if (last) {
+      // step of heads + run grows from one piece to the next: it numbers the pieces
+      const long long piece = ((long long)at.b * a.per + at.j + run) * WARPS + warp;
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -642,7 +751,7 @@ __global__ void __launch_bounds__(32 * NWARP, 1)
           l += __shfl_xor_sync(0xffffffffu, l, 8);
           l += __shfl_xor_sync(0xffffffffu, l, 16);
           if (qf.row[nt][e] >= a.R) continue;
-          const long long row = slot * (8 * NT) + nt * 8 + 2 * c + e;
+          const long long row = piece * (8 * NT) + nt * 8 + 2 * c + e;
           if (g == 0) __stcg(a.part_ml + row, make_float2(ok ? st.m[nt][e] : -INFINITY, l));
           float4* const dst = reinterpret_cast<float4*>(a.part_o + row * HD + 16 * g);
 #pragma unroll
@@ -650,13 +759,13 @@ __global__ void __launch_bounds__(32 * NWARP, 1)
             __stcg(dst + j / 2, make_float4(st.o[j][nt][e], st.o[j][nt][2 + e], st.o[j + 1][nt][e], st.o[j + 1][nt][2 + e]));
         }
       }
-      if (i + 1 < n) {
-        at = then;
-        enter();
-      }
     }
-    at = then;
-    sc = sc_next;
+    if (!more) break;
+    at = ahead;
+    more = ahead.next(a, step, start);
+    if (more && ok) fetch(s, false);
+    turn();
+    if (last) enter();
   }
   if (!ok) {  // let this warp's copies in flight land before the shared memory goes away
     const long long t0 = clock64();
@@ -664,57 +773,67 @@ __global__ void __launch_bounds__(32 * NWARP, 1)
   }
 }
 
-// Rows of the output: each row's partial results in run order, `merge_per_row` warps a row (each a
-// contiguous part of them), four dims a lane.
+// Rows of the output: each row's partial results in the order of runs and warps, `merge_per_row` warps a
+// row (each a contiguous part of them), four dims a lane, eight partials in flight.
 template <int NT>
-__global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(DecArgs a) {
+__global__ void __launch_bounds__(32 * MERGE_WARPS, 2) cache_merge_kernel(const __grid_constant__ DecArgs a) {
   __shared__ float4 so[MERGE_WARPS][32];
   __shared__ float2 sml[MERGE_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per = a.merge_per_row, rows_here = MERGE_WARPS / per, part = warp % per;
-  const long long rows = (long long)a.B * a.Hk * a.R;
-  const long long row = (long long)blockIdx.x * rows_here + warp / per;  // (b * Hk + h) * R + r
+  const int per = a.merge_per_row, rows_here = blockDim.x / 32 / per, part = warp % per;
+  const int row = blockIdx.x * rows_here + warp / per, rows = a.B * a.Hk * a.R;  // (b * Hk + h) * R + r
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float M = -INFINITY, L = 0.f;
   int r = 0, h = 0, b = 0, len = 0;
+  pdl_wait();
+  pdl_launch();
   if (row < rows) {
-    r = (int)(row % a.R);
-    h = (int)(row / a.R % a.Hk);
-    b = (int)(row / a.R / a.Hk);
+    r = row % a.R;
+    h = row / a.R % a.Hk;
+    b = row / a.R / a.Hk;
     len = seq_len(a, b);
-    const int n = (len + KT - 1) / KT, hg = h * a.n_group + r / (8 * NT);
-    const Runs runs(tiles_before(a, a.B, lane) * a.Hk * a.n_group, a.runs);
-    const long long f = tiles_before(a, b, lane) * a.Hk * a.n_group + (long long)hg * n;
-    pdl_wait();
+    const int hg = h * a.n_group + r / (8 * NT), j = hg / a.heads, n = (len + UNIT - 1) / UNIT;
+    const Runs runs(units_before(a, a.B, lane), a.runs);
+    const int f = units_before(a, b, lane) + j * n;
     if (n > 0) {
-      const int r0 = runs.owner(f), r1 = runs.owner(f + n - 1) + 1, cnt = r1 - r0;
-      const int lo = r0 + cnt * part / per, hi = r0 + cnt * (part + 1) / per;
-      const long long base = ((long long)b * a.Hk * a.n_group + hg) * (8 * NT) + r % (8 * NT);
-      for (int i0 = lo; i0 < hi; i0 += 32) {  // references of 32 partials at once, then their rows
-        const float2 ml = i0 + lane < hi ? __ldcg(a.part_ml + base + (long long)(i0 + lane) * (8 * NT)) : make_float2(-INFINITY, 0.f);
+      const int r0 = runs.owner(f), cnt = (runs.owner(f + n - 1) + 1 - r0) * a.keys;
+      const int lo = cnt * part / per, hi = cnt * (part + 1) / per;
+      // partial i: run r0 + i / keys, the warp of this head with key tiles i % keys
+      const long long base = (((long long)b * a.per + j + r0) * WARPS + hg - j * a.heads) * (8 * NT) + r % (8 * NT);
+      const int stride = a.heads * 8 * NT;
+      for (int i0 = lo; i0 < hi; i0 += 8) {
+        float4 v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+          v[i] = __ldcg(reinterpret_cast<const float4*>(a.part_o + (base + (long long)min(i0 + i, hi - 1) * stride) * HD) + lane);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        const int mine = i0 + lane;
+        if (lane < 8 && mine < hi) {
+          // the warp wrote a partial if the run's part of the head reaches its first tile
+          const int run = r0 + mine / a.keys, from = max(f, runs.begin(run)), to = min(f + n, runs.begin(run + 1));
+          if (from + mine % a.keys * units_of_tile(NT) < to) ml = __ldcg(a.part_ml + base + (long long)mine * stride);
+        }
         float top = ml.x;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = 4; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = __shfl_sync(0xffffffffu, top, 0);
         const float m_new = max_nan(M, top), ref = m_new == -INFINITY ? 0.f : m_new;
         const float al = M == -INFINITY ? 0.f : ex2f(M - ref), w = ml.x == -INFINITY ? 0.f : ex2f(ml.x - ref);
-        float l = w * ml.y;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         M = m_new;
-        L = L * al + l;
+        L *= al;
         acc.x *= al;
         acc.y *= al;
         acc.z *= al;
         acc.w *= al;
-        const int m = min(32, hi - i0);
-#pragma unroll 4
-        for (int i = 0; i < m; i++) {
-          const float wi = __shfl_sync(0xffffffffu, w, i);
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + (base + (long long)(i0 + i) * (8 * NT)) * HD) + lane);
-          acc.x = fmaf(wi, v.x, acc.x);
-          acc.y = fmaf(wi, v.y, acc.y);
-          acc.z = fmaf(wi, v.z, acc.z);
-          acc.w = fmaf(wi, v.w, acc.w);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float wi = __shfl_sync(0xffffffffu, w, i), li = __shfl_sync(0xffffffffu, ml.y, i);
+          if (wi == 0.f) continue;  // nothing was written there, or nothing of it counts
+          L = fmaf(wi, li, L);
+          acc.x = fmaf(wi, v[i].x, acc.x);
+          acc.y = fmaf(wi, v[i].y, acc.y);
+          acc.z = fmaf(wi, v[i].z, acc.z);
+          acc.w = fmaf(wi, v[i].w, acc.w);
         }
       }
     }
@@ -750,9 +869,15 @@ int rows_of(const CacheDecodeProblem& p) { return p.Sq * (p.Hq / p.Hk); }
 int col_tiles(const CacheDecodeProblem& p) { return rows_of(p) > 8 ? 2 : 1; }
 int groups_of(const CacheDecodeProblem& p) { return (rows_of(p) + 8 * col_tiles(p) - 1) / (8 * col_tiles(p)); }
 
-long long units_of(const CacheDecodeProblem& p) { return (long long)p.B * p.Hk * groups_of(p); }
-int runs_of(const CacheDecodeProblem& p) { return p.num_sms * NWARP; }
-long long partials_of(const CacheDecodeProblem& p) { return (units_of(p) + runs_of(p)) * 8 * col_tiles(p); }
+// as many (head, group) units side by side as divide their number
+int heads_of(const CacheDecodeProblem& p) {
+  const int u = p.Hk * groups_of(p);
+  for (int h = WARPS; h > 1; h /= 2)
+    if (u % h == 0) return h;
+  return 1;
+}
+long long head_steps_of(const CacheDecodeProblem& p) { return (long long)p.B * (p.Hk * groups_of(p) / heads_of(p)); }
+long long partials_of(const CacheDecodeProblem& p) { return (head_steps_of(p) + p.num_sms) * WARPS * 8 * col_tiles(p); }
 
 // One map of a cache side: [128 bytes][heads][tokens][sequences]. A broadcast dimension (stride 0)
 // is mapped with one entry.
@@ -760,33 +885,25 @@ bool side_map(CUtensorMap* m, const CacheSide& s, const CacheDecodeProblem& p, i
   one_b = p.B == 1 || s.c_b == 0;
   one_h = p.Hk == 1 || s.c_h == 0;
   return make_tmap_4d_u8(m, s.codes, HD, one_h ? 1 : p.Hk, p.L, one_b ? 1 : p.B, one_h ? HD : s.c_h,
-                         p.L == 1 ? HD : s.c_tok, one_b ? HD : s.c_b, HD, 1, KT, 1);
+                         p.L == 1 ? HD : s.c_tok, one_b ? HD : s.c_b, HD, 1, UNIT, 1);
 }
 
 template <int NT, int FMT>
 cudaError_t launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecArgs& a, int sms, cudaStream_t stream) {
-  const int smem = (int)sizeof(DecSmem) + 1024;
+  const int smem = (int)sizeof(DecSmem<NT>) + 1024;
   static bool attr = false;
   if (!attr) {
     const cudaError_t e = cudaFuncSetAttribute(cache_decode_kernel<NT, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     attr = true;
   }
-  cache_decode_kernel<NT, FMT><<<sms, 32 * NWARP, smem, stream>>>(tk, tv, a);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e =
+      launch_overlapped(cache_decode_kernel<NT, FMT>, (unsigned)sms, 32 * WARPS, smem, stream, tk, tv, a);
   if (e != cudaSuccess) return e;
-  // the merge may start while the first kernel's last CTAs run; it waits for them before it reads
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  const long long rows = (long long)a.B * a.Hk * a.R;
-  cfg.gridDim = dim3((unsigned)((rows * a.merge_per_row + MERGE_WARPS - 1) / MERGE_WARPS));
-  cfg.blockDim = dim3(32 * MERGE_WARPS);
-  cfg.stream = stream;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, cache_merge_kernel<NT>, a);
+  // CTAs of four warps, or of one row's where that is more: small ones fill the SMs evenly
+  const int warps = std::max(4, a.merge_per_row), rows_here = warps / a.merge_per_row;
+  const int rows = a.B * a.Hk * a.R;
+  return launch_overlapped(cache_merge_kernel<NT>, (unsigned)((rows + rows_here - 1) / rows_here), 32 * warps, 0, stream, a);
 }
 
 }  // namespace
@@ -849,16 +966,19 @@ cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream) {
   a.len_all = p.len_all;
   a.max_len = p.max_len;
   a.scale_log2 = p.scale * 1.4426950408889634f;
-  a.runs = runs_of(p);
+  a.heads = heads_of(p);
+  a.keys = WARPS / a.heads;
+  a.per = p.Hk * a.n_group / a.heads;
+  a.runs = p.num_sms;
   const long long rows = (long long)p.B * p.Hk * a.R;
-  // units, runs and rows are numbered in 32 bits on the way
-  if (rows > 0x3fffffffLL || units_of(p) > 0x3fffffffLL || p.B > (1 << 24)) return cudaErrorInvalidValue;
+  const long long units = head_steps_of(p) * ((p.max_len + UNIT - 1) / UNIT);
+  if (rows > 0x3fffffffLL || units > 0x3fffffffLL) return cudaErrorInvalidValue;  // both are numbered in 32 bits
   if (p.scratch == nullptr) return cudaErrorInvalidValue;
   a.part_o = p.scratch;
   a.part_ml = reinterpret_cast<float2*>(p.scratch + (size_t)partials_of(p) * HD);
-  // a row has about runs / units partials; warps that share it take a few each
-  const long long expect = a.runs / units_of(p);
-  a.merge_per_row = expect >= 64 ? 8 : expect >= 16 ? 4 : expect >= 8 ? 2 : 1;
+  // a row has at most about this many partials; warps that share it take a few each
+  const long long expect = (a.runs / head_steps_of(p) + 1) * a.keys;
+  a.merge_per_row = expect >= 64 ? 16 : expect >= 32 ? 8 : expect >= 16 ? 4 : expect >= 8 ? 2 : 1;
   CUtensorMap tk, tv;
   if (p.L > 0 && (!side_map(&tk, p.side[0], p, a.one_b[0], a.one_h[0]) || !side_map(&tv, p.side[1], p, a.one_b[1], a.one_h[1])))
     return cudaErrorInvalidValue;
