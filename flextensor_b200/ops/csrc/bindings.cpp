@@ -278,7 +278,7 @@ void decode_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, Tenso
 // refused call says why on any machine.
 constexpr int64_t kHead = 128;
 
-bool on_16_bytes(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+bool on_16_bytes(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0; }
 
 void check_cache(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, int64_t block, const char* op) {
   TORCH_CHECK(kc.dim() == 4 && kc.size(3) == kHead && vc.sizes() == kc.sizes(), op,
@@ -462,14 +462,20 @@ Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tenso
   const bool res = residual && residual->defined();
   if (res) matrix(*residual, "residual", T, D);
   ft::MoeDecodeProblem p;
-  for (int64_t e = 0; e < E; e++) {
-    matrix(gate_up[e], "w_gate_up", 2 * F, D);
-    matrix(down[e], "w_down", D, F);
-    TORCH_CHECK(gate_up[e].stride(0) == gate_up[0].stride(0) && down[e].stride(0) == down[0].stride(0), op,
-                ": the experts' weights must have one row stride");
-    p.w_gate_up[e] = reinterpret_cast<const __nv_bfloat16*>(gate_up[e].data_ptr());
-    p.w_down[e] = reinterpret_cast<const __nv_bfloat16*>(down[e].data_ptr());
-  }
+  // many experts: the quick form of matrix() and of the device check, which say what is wrong if it fails
+  auto weights = [&](const std::vector<Tensor>& w, const char* name, int64_t r, int64_t c, const __nv_bfloat16** to) {
+    for (int64_t e = 0; e < E; e++) {
+      const Tensor& t = w[e];
+      const auto size = t.sizes(), stride = t.strides();
+      if (t.scalar_type() != at::kBFloat16 || size.size() != 2 || size[0] != r || size[1] != c || stride[1] != 1 ||
+          stride[0] % 8 != 0 || !on_16_bytes(t))
+        matrix(t, name, r, c);
+      TORCH_CHECK(stride[0] == w[0].stride(0), op, ": the experts' weights must have one row stride");
+      to[e] = reinterpret_cast<const __nv_bfloat16*>(t.const_data_ptr());
+    }
+  };
+  weights(gate_up, "w_gate_up", 2 * F, D, p.w_gate_up);
+  weights(down, "w_down", D, F, p.w_down);
   TORCH_CHECK(at::has_internal_overlap(out) != at::MemOverlap::Yes, op, ": out must not overlap itself");
   at::assert_no_partial_overlap(out, x);
   if (res) at::assert_no_partial_overlap(out, *residual);

@@ -4,11 +4,16 @@
 //
 // Every weight of every expert that a token chose is read once and meets a handful of tokens, so
 // the layer is bound by the HBM stream of the weights. Launches:
-//   route    one CTA a token: logits in fp32, top-k, softmax;
+//   logits   x router^T in fp32, one CTA per expert and four tokens;
 //   gate/up  D[weight row, token] = W x^T on tcgen05 (weights are the 128-row operand, the tokens
-//            the narrow one), SwiGLU on the accumulator, h in bf16;
-//   down     the same product with h, fp32 partial sums;
+//            the narrow one), SwiGLU on the accumulator, h as a sum of two bf16 numbers;
+//   down     the same product with both parts of h, fp32 partial sums;
 //   combine  the partial sums of a token's experts with their weights and the residual.
+// Each may start while the one before it ends (programmatic serialization). The choice of experts
+// is a few hundred numbers, so every CTA of both products makes it for itself from the logits;
+// the down product fills its stages with weights before it waits for h.
+// h in one bf16 number would add an error as large as the output's own rounding; its second half
+// costs one more MMA per tile and a few KB from L2.
 // The two products split the stream of 128-row x 64-column weight tiles of all chosen experts into
 // equal contiguous runs, one per CTA (a CTA per SM), whatever the expert and tile boundaries: every
 // SM reads the same number of bytes. A weight tile that several CTAs share part of is summed in
@@ -53,23 +58,25 @@ struct Args {
   long long ldres;
   __nv_bfloat16* out;
   long long ldo;
-  int* ids;                             // [slots] expert of each pair
+  float* logits;                        // [T, E]
   float* wts;                           // [slots]
   int* place;                           // [slots] slot | position of its expert among the chosen << 16; [slots] their number
   unsigned int* done;                   // per weight tile of the gate/up product: segments finished
   int n_done;
-  __nv_bfloat16* h;                     // [slots, F], slots ordered by expert, then token
+  __nv_bfloat16* h;                     // [2][slots, F], high and low parts, slots ordered by expert, then token
   float* part;                          // gate/up: [2 * CTAs][cols][128] partial tiles
   float* y;                             // down: [splits][slots][D] partial sums
   int cols;                             // token columns of an MMA: T rounded up to 16
-  int stages, stage_bytes;
-  int one_map;                          // the experts' weights are equally spaced: one tensor map
+  int one_map;                          // one tensor map for all experts
 };
 
 template <int N>
 struct Maps {
   CUtensorMap w[N];
 };
+
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // A wait that runs out (2 s) is recorded; the caller then skips its work but keeps its barriers.
 __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t phase) {
@@ -86,93 +93,132 @@ __device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t phase) {
 }
 
 // ------------------------------------------------------------------------------------ routing
-constexpr int ROUTE_WARPS = 8;
+constexpr int LOGIT_WARPS = 8;
+constexpr int LOGIT_TOKENS = 4;
 
-__global__ void __launch_bounds__(32 * ROUTE_WARPS) moe_route_kernel(Args a) {
-  __shared__ float logit[MAX_E];
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < a.n_done; i += gridDim.x * blockDim.x) a.done[i] = 0;
-  const uint4* x = reinterpret_cast<const uint4*>(a.x + t * a.ldx);
-  for (int e = warp; e < a.E; e += ROUTE_WARPS) {
-    const uint4* r = reinterpret_cast<const uint4*>(a.router + e * a.ldr);
-    float s = 0.f;
-#pragma unroll 4
-    for (int i = lane; i < a.D / 8; i += 32) {
-      const uint4 u = x[i], v = r[i];
-      const uint32_t uw[4] = {u.x, u.y, u.z, u.w}, vw[4] = {v.x, v.y, v.z, v.w};
+// CTA (expert, four tokens): the router's row is read once for the four
+__global__ void __launch_bounds__(32 * LOGIT_WARPS) moe_logits_kernel(const __grid_constant__ Args a) {
+  __shared__ float part[LOGIT_WARPS][LOGIT_TOKENS];
+  const int e = blockIdx.x, t0 = blockIdx.y * LOGIT_TOKENS, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch();
+  const int id = (blockIdx.y * gridDim.x + blockIdx.x) * blockDim.x + threadIdx.x;
+  for (int i = id; i < a.n_done; i += gridDim.x * gridDim.y * blockDim.x) a.done[i] = 0;
+  const uint4* const r = reinterpret_cast<const uint4*>(a.router + e * a.ldr);
+  float s[LOGIT_TOKENS] = {};
+#pragma unroll 2
+  for (int i = threadIdx.x; i < a.D / 8; i += 32 * LOGIT_WARPS) {
+    const uint4 v = r[i];
+    const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int t = 0; t < LOGIT_TOKENS; t++) {
+      const uint4 u = reinterpret_cast<const uint4*>(a.x + min(t0 + t, a.T - 1) * a.ldx)[i];
+      const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        s = fmaf(__uint_as_float(uw[j] << 16), __uint_as_float(vw[j] << 16), s);
-        s = fmaf(__uint_as_float(uw[j] & 0xffff0000u), __uint_as_float(vw[j] & 0xffff0000u), s);
+        s[t] = fmaf(__uint_as_float(uw[j] << 16), __uint_as_float(vw[j] << 16), s[t]);
+        s[t] = fmaf(__uint_as_float(uw[j] & 0xffff0000u), __uint_as_float(vw[j] & 0xffff0000u), s[t]);
       }
     }
+  }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) logit[e] = s;
+  for (int t = 0; t < LOGIT_TOKENS; t++) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s[t] += __shfl_xor_sync(0xffffffffu, s[t], o);
+    if (lane == 0) part[warp][t] = s[t];
   }
   __syncthreads();
-  if (warp != 0) return;
-  // top-k by repeated maximum; equal logits go to the lower expert, NaN counts as the largest
-  float mine = 0.f, top = 0.f, sum = 0.f;
-  int mine_e = 0;
-  unsigned int taken = 0;  // this lane's experts lane, lane + 32, ...
+  if (threadIdx.x < LOGIT_TOKENS && t0 + threadIdx.x < a.T) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < LOGIT_WARPS; w++) v += part[w][threadIdx.x];
+    a.logits[(t0 + threadIdx.x) * a.E + e] = v;
+  }
+}
+
+// A token's experts by repeated maximum, by a whole warp: equal logits go to the lower expert, NaN
+// counts as the largest. Lane k < topk gets choice k and its weight.
+__device__ __forceinline__ void choose(const Args& a, int t, int lane, int& mine_e, float& mine_w) {
+  constexpr int PER = MAX_E / 32;
+  float v[PER];
+  uint32_t key[PER];
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    v[i] = i * 32 + lane < a.E ? __ldcg(a.logits + t * a.E + i * 32 + lane) : 0.f;
+    const uint32_t b = __float_as_uint(v[i]);
+    key[i] = v[i] != v[i] ? 0xffffffffu : (v[i] == 0.f ? 0x80000000u : (b & 0x80000000u ? ~b : b | 0x80000000u));
+    if (i * 32 + lane >= a.E) key[i] = 0;  // below every number: -infinity is 0x007fffff
+  }
+  float top = 0.f, sum = 0.f, mine = 0.f;
+  mine_e = 0;
   for (int k = 0; k < a.topk; k++) {
     uint32_t best = 0;
-    int be = MAX_E;
-    for (int i = 0; i * 32 + lane < a.E; i++) {
-      if (taken >> i & 1) continue;
-      const float v = logit[i * 32 + lane];
-      const uint32_t b = __float_as_uint(v);
-      const uint32_t key = v != v ? 0xffffffffu : (v == 0.f ? 0x80000000u : (b & 0x80000000u ? ~b : b | 0x80000000u));
-      if (key > best || be == MAX_E) {
-        best = key;
-        be = i * 32 + lane;
-      }
-    }
-    const uint32_t m = __reduce_max_sync(0xffffffffu, be < MAX_E ? best : 0u);
-    const int e = (int)__reduce_min_sync(0xffffffffu, be < MAX_E && best == m ? (unsigned)be : (unsigned)MAX_E);
-    if ((e & 31) == lane) taken |= 1u << (e >> 5);
-    const float v = logit[e];
-    if (k == 0) top = v;
-    const float p = expf(v - top);
+#pragma unroll
+    for (int i = 0; i < PER; i++) best = max(best, key[i]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    unsigned int e = MAX_E;
+    float val = 0.f;
+#pragma unroll
+    for (int i = PER - 1; i >= 0; i--)
+      if (key[i] == best) e = i * 32 + lane, val = v[i];
+    const unsigned int chosen = __reduce_min_sync(0xffffffffu, e);
+    val = __shfl_sync(0xffffffffu, val, chosen & 31);
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+      if (i * 32 + lane == chosen) key[i] = 0;
+    if (k == 0) top = val;
+    const float p = expf(val - top);
     sum += p;
     if (lane == k) {
       mine = p;
-      mine_e = e;
+      mine_e = (int)chosen;
     }
   }
-  if (lane < a.topk) {
-    a.ids[t * a.topk + lane] = mine_e;
-    a.wts[t * a.topk + lane] = mine / sum;
-  }
+  mine_w = mine / sum;
 }
 
 // ------------------------------------------------------------------------------------ the products
 struct Tables {
   short id[MAX_SLOTS];        // expert of each (token, choice) pair
   short pair[MAX_SLOTS];      // pairs ordered by expert, then token
+  short token[MAX_SLOTS];     // and their tokens
   short off[MAX_E + 1];       // first slot of each expert
   short act[MAX_E];           // the experts that were chosen
   int n_act;
+  int most;                   // tokens of the expert with the most
 };
 
-// The stream of weight tiles: item = (chosen expert, row tile), KC tiles along the inner dimension.
+// The stream of weight tiles (fewer than 2^31: a tile is 16 KB): item = (chosen expert, row tile), kc
+// tiles along the inner dimension. CTA c takes tiles [begin(c), begin(c + 1)), the first `rem` CTAs one
+// more than the others.
 struct Stream {
-  int rt, kc, ctas;
-  long long total;
+  int rt, kc, ctas, base, rem;
   __device__ __forceinline__ Stream(int n_act, int row_tiles, int k_chunks, int grid) : rt(row_tiles), kc(k_chunks) {
-    total = (long long)n_act * row_tiles * k_chunks;
-    ctas = (int)min((long long)grid, max(1LL, total / MIN_CHUNKS));
+    const int total = n_act * row_tiles * k_chunks;
+    ctas = min(grid, max(1, total / MIN_CHUNKS));
+    base = total / ctas;
+    rem = total - base * ctas;
   }
-  __device__ __forceinline__ long long begin(int c) const { return total * c / ctas; }
+  __device__ __forceinline__ int begin(int c) const { return c * base + min(c, rem); }
   // the CTA whose run holds tile i
-  __device__ __forceinline__ int owner(long long i) const { return (int)(((i + 1) * ctas - 1) / total); }
+  __device__ __forceinline__ int owner(int i) const {
+    const int longer = rem * (base + 1);
+    return i < longer ? i / (base + 1) : rem + (i - longer) / base;
+  }
 };
 
-// expert tables of every CTA, from the router's choices (a few hundred numbers)
-__device__ void build_tables(Tables& tb, const Args& a) {
+// expert tables of every CTA, from the logits
+__device__ void build_tables(Tables& tb, const Args& a, bool keep_weights) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int i = threadIdx.x; i < a.slots; i += NTHREADS) tb.id[i] = (short)__ldcg(a.ids + i);
+  for (int t = warp; t < a.T; t += NTHREADS / 32) {
+    int e;
+    float w;
+    choose(a, t, lane, e, w);
+    if (lane < a.topk) {
+      tb.id[t * a.topk + lane] = (short)e;
+      if (keep_weights) a.wts[t * a.topk + lane] = w;
+    }
+  }
   __syncthreads();
   for (int e = warp; e < a.E; e += NTHREADS / 32) {
     int n = 0;
@@ -182,13 +228,14 @@ __device__ void build_tables(Tables& tb, const Args& a) {
   __syncthreads();
   if (warp == 0) {
     constexpr int PER = MAX_E / 32;
-    int n[PER], sum = 0, used = 0;
+    int n[PER], sum = 0, used = 0, most = 0;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
       const int e = lane * PER + i;
       n[i] = e < a.E ? tb.off[e + 1] : 0;
       sum += n[i];
       used += n[i] > 0;
+      most = max(most, n[i]);
     }
     int s = sum, u = used;
 #pragma unroll
@@ -196,7 +243,8 @@ __device__ void build_tables(Tables& tb, const Args& a) {
       const int sv = __shfl_up_sync(0xffffffffu, s, o), uv = __shfl_up_sync(0xffffffffu, u, o);
       if (lane >= o) s += sv, u += uv;
     }
-    if (lane == 31) tb.n_act = u;
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 31) tb.n_act = u, tb.most = most;
     if (lane == 0) tb.off[0] = 0;
     s -= sum;
     u -= used;
@@ -216,7 +264,11 @@ __device__ void build_tables(Tables& tb, const Args& a) {
     for (int i = 0; i < a.slots; i += 32) {
       const bool hit = i + lane < a.slots && tb.id[i + lane] == e;
       const unsigned int m = __ballot_sync(0xffffffffu, hit);
-      if (hit) tb.pair[at + __popc(m & ((1u << lane) - 1))] = (short)(i + lane);
+      if (hit) {
+        const int to = at + __popc(m & ((1u << lane) - 1));
+        tb.pair[to] = (short)(i + lane);
+        tb.token[to] = (short)((i + lane) / a.topk);
+      }
       at += __popc(m);
     }
   }
@@ -238,14 +290,14 @@ __device__ __forceinline__ void tmem_ld_x1(uint32_t taddr, uint32_t& r) {
 // K = F, D weight rows).
 template <bool UP, int N_MAPS>
 __global__ void __launch_bounds__(NTHREADS, 1)
-    moe_product_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ Maps<N_MAPS> maps,
-                       const __grid_constant__ Args a) {
+    moe_product_kernel(const __grid_constant__ CUtensorMap tm_b, const __grid_constant__ CUtensorMap tm_lo,
+                       const __grid_constant__ Maps<N_MAPS> maps, const __grid_constant__ Args a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ Ctrl sm;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < a.stages; s++) {
+    for (int s = 0; s < MAX_STAGES; s++) {
       mbar_init(&sm.full[s], 1);
       mbar_init(&sm.empty[s], 1);
     }
@@ -260,7 +312,13 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     tmem_alloc(&sm.tmem, TMEM_COLS);
     tmem_relinquish();
   }
-  build_tables(sm.tb, a);
+  // The logits are there: the gate/up product waits for their kernel, and the down product starts
+  // only after every CTA of the gate/up product has done so.
+  if (UP) {
+    pdl_wait();
+    pdl_launch();
+  }
+  build_tables(sm.tb, a, UP && blockIdx.x == 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -268,8 +326,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   const uint32_t tmem_base = sm.tmem;
   const int rows = UP ? 2 * a.F : a.D, K = UP ? a.D : a.F;
   const Stream st(tb.n_act, (rows + BM - 1) / BM, (K + BK - 1) / BK, gridDim.x);
+  // a stage holds a weight tile and the token columns that go with it, for the down product both parts
+  // of the rows of the largest group
+  const int cols = UP ? a.cols : (tb.most + 15) / 16 * 16, stage_bytes = A_BYTES + cols * 128 * (UP ? 1 : 2);
+  const int stages = min(MAX_STAGES, RING_BUDGET / stage_bytes);
   const int cta = blockIdx.x;
-  const long long begin = cta < st.ctas ? st.begin(cta) : 0, end = cta < st.ctas ? st.begin(cta + 1) : 0;
+  const int begin = cta < st.ctas ? st.begin(cta) : 0, end = cta < st.ctas ? st.begin(cta + 1) : 0;
 
   if (UP && cta == 0) {  // where each pair's row of h and of the partial sums is, for the combine kernel
     for (int ai = warp; ai < tb.n_act; ai += NTHREADS / 32)
@@ -279,28 +341,68 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
   if (warp == 0) {
     if (elect_one()) {
-      const uint32_t tile_bytes = A_BYTES + a.cols * BK * 2;
       int s = 0;
       uint32_t ph = 0, pend = 0, pend_ph = 0;
       bool ok = true;
-      for (long long i = begin; i < end && ok;) {
-        const long long item = i / st.kc;
-        const int ai = (int)(item / st.rt), rt = (int)(item % st.rt), e = tb.act[ai];
-        const long long stop = min(end, (item + 1) * st.kc);
-        const CUtensorMap* tm_a = &maps.w[a.one_map ? 0 : e];
-        const int z = a.one_map ? e : 0, brow = UP ? 0 : tb.off[e];
-        for (int kb = (int)(i - item * st.kc); i < stop; i++, kb++) {
+      // weights of tile i of the run, tokens of it: a down tile takes both parts of the expert's rows of h, 16 a copy
+      auto place_of = [&](int i, int& ai, int& rt, int& kb) {
+        const int item = i / st.kc;
+        ai = item / st.rt;
+        rt = item - ai * st.rt;
+        kb = i - item * st.kc;
+      };
+      auto tokens_bytes = [&](int e) {
+        return UP ? cols * 128 : (tb.off[e + 1] - tb.off[e] + 15) / 16 * (2 * 16 * 128);
+      };
+      auto load_weights = [&](int s, int e, int rt, int kb) {
+        mbar_arrive_expect_tx(&sm.full[s], A_BYTES + tokens_bytes(e));
+        tma_load_3d(ring + (size_t)s * stage_bytes, &maps.w[a.one_map ? 0 : e], &sm.full[s], kb * BK, rt * BM, a.one_map ? e : 0);
+      };
+      auto load_tokens = [&](int s, int e, int kb) {
+        uint8_t* const dst = ring + (size_t)s * stage_bytes + A_BYTES;
+        if (UP) {
+          tma_load_2d(dst, &tm_b, &sm.full[s], kb * BK, 0);
+        } else {
+          for (int r = tb.off[e], at = 0; r < tb.off[e + 1]; r += 16, at += 16 * 128) {
+            tma_load_2d(dst + at, &tm_b, &sm.full[s], kb * BK, r);
+            tma_load_2d(dst + cols * 128 + at, &tm_lo, &sm.full[s], kb * BK, r);
+          }
+        }
+      };
+      int i = begin;
+      if (!UP) {  // the first stages' weights do not depend on h
+        const int n = min(stages, end - begin);
+        int ai, rt, kb;
+        for (int b = 0; b < n; b++) {
+          place_of(begin + b, ai, rt, kb);
+          load_weights(b, tb.act[ai], rt, kb);
+        }
+        pdl_wait();
+        fence_proxy_async_global();
+        for (int b = 0; b < n; b++) {
+          place_of(begin + b, ai, rt, kb);
+          load_tokens(b, tb.act[ai], kb);
+        }
+        i += n;
+        pend = (1u << n) - 1;
+        s = n % stages;
+        ph = n == stages;
+      }
+      while (i < end && ok) {
+        int ai, rt, kb;
+        place_of(i, ai, rt, kb);
+        const int e = tb.act[ai];
+        const int stop = min(end, i - kb + st.kc);
+        for (; i < stop; i++, kb++) {
           if (!bounded_wait(&sm.empty[s], ph ^ 1)) {
             ok = false;
             break;
           }
-          uint8_t* const dst = ring + (size_t)s * a.stage_bytes;
-          mbar_arrive_expect_tx(&sm.full[s], tile_bytes);
-          tma_load_3d(dst, tm_a, &sm.full[s], kb * BK, rt * BM, z);
-          tma_load_2d(dst + A_BYTES, &tm_b, &sm.full[s], kb * BK, brow);
+          load_weights(s, e, rt, kb);
+          load_tokens(s, e, kb);
           pend |= 1u << s;
           pend_ph = (pend_ph & ~(1u << s)) | (ph << s);
-          if (++s == a.stages) {
+          if (++s == stages) {
             s = 0;
             ph ^= 1;
           }
@@ -308,7 +410,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
       if (!ok) {  // let the copies in flight land before the CTA's shared memory goes away
         const long long t0 = clock64();
-        for (int b = 0; b < a.stages; b++)
+        for (int b = 0; b < stages; b++)
           if (pend >> b & 1)
             while (!mbar_try_wait(smem_u32(&sm.full[b]), (pend_ph >> b) & 1) &&
                    (unsigned long long)(clock64() - t0) < FT_WAIT_LIMIT_CYCLES / 4) {
@@ -317,28 +419,36 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     }
   } else if (warp == 1) {
     if (elect_one()) {
-      const uint32_t idesc = umma_idesc_bf16_f32(BM, 0) | ((uint32_t)(a.cols >> 3) << 17);
       int s = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
-      for (long long i = begin; i < end && ok;) {
-        const long long first = i, stop = min(end, (i / st.kc + 1) * st.kc);
+      for (int i = begin; i < end && ok;) {
+        const int first = i, item = i / st.kc, stop = min(end, (item + 1) * st.kc);
         if (!bounded_wait(&sm.tempty[acc], acc_ph ^ 1)) break;
         tc_fence_after();
         const uint32_t dt = tmem_base + acc * MAX_T;
+        const int e = tb.act[item / st.rt];
+        const int here = UP ? cols : (tb.off[e + 1] - tb.off[e] + 15) / 16 * 16;
+        const uint32_t idesc = umma_idesc_bf16_f32(BM, 0) | ((uint32_t)(here >> 3) << 17);
         for (; i < stop; i++) {
           if (!bounded_wait(&sm.full[s], ph)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a0 = smem_u32(ring) + s * a.stage_bytes, b0 = a0 + A_BYTES;
+          const uint32_t a0 = smem_u32(ring) + s * stage_bytes, b0 = a0 + A_BYTES;
 #pragma unroll
           for (int k = 0; k < BK / 16; k++)
             umma_bf16_ss(dt, umma_desc_kmajor_sw128(a0 + k * 32), umma_desc_kmajor_sw128(b0 + k * 32), idesc,
                          i != first || k != 0);
+          if constexpr (!UP) {
+            const uint32_t l0 = b0 + cols * 128;
+#pragma unroll
+            for (int k = 0; k < BK / 16; k++)
+              umma_bf16_ss(dt, umma_desc_kmajor_sw128(a0 + k * 32), umma_desc_kmajor_sw128(l0 + k * 32), idesc, 1);
+          }
           umma_commit(&sm.empty[s]);
-          if (++s == a.stages) {
+          if (++s == stages) {
             s = 0;
             ph ^= 1;
           }
@@ -357,13 +467,17 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       }
     }
   } else {
+    if (!UP) {
+      pdl_wait();  // the partial sums' memory may be in use until here
+      pdl_launch();
+    }
     const int q = warp & 3, row_in = q * 32 + lane;
     int acc = 0;
     uint32_t acc_ph = 0;
     bool ok = true;  // after a wait that ran out, no accumulator is read, but every barrier below is kept
-    for (long long i = begin; i < end;) {
-      const long long item = i / st.kc, stop = min(end, (item + 1) * st.kc);
-      const int ai = (int)(item / st.rt), row = (int)(item % st.rt) * BM + row_in, e = tb.act[ai];
+    for (int i = begin; i < end;) {
+      const int item = i / st.kc, stop = min(end, (item + 1) * st.kc);
+      const int ai = item / st.rt, row = (item - ai * st.rt) * BM + row_in, e = tb.act[ai];
       const int off = tb.off[e], n = tb.off[e + 1] - off;
       const bool whole = stop - i == st.kc;
       if (ok) ok = __all_sync(0xffffffffu, bounded_wait(&sm.tfull[acc], acc_ph));
@@ -377,7 +491,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 #pragma unroll
           for (int u = 0; u < 8; u++) {
             const int j = min(j0 + u, n - 1);
-            tmem_ld_x1(src + (UP ? tb.pair[off + j] / a.topk : j), v[u]);
+            tmem_ld_x1(src + (UP ? tb.token[off + j] : j), v[u]);
           }
           tmem_ld_wait();
 #pragma unroll
@@ -390,8 +504,16 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         const float up = __shfl_down_sync(0xffffffffu, v, 1);
         const float h = v / (1.f + __expf(-v)) * up;
         const float next = __shfl_down_sync(0xffffffffu, h, 2);
-        if ((lane & 3) == 0 && row < rows)
-          *reinterpret_cast<uint32_t*>(a.h + (long long)(off + j) * a.F + row / 2) = pack_bf16x2(h, next);
+        if ((lane & 3) == 0 && row < rows) {
+          const uint32_t hi = pack_bf16x2(h, next);
+          auto rest = [](float x, uint32_t bits) {  // an infinite high part is the whole of it
+            return (bits & 0x7f800000u) == 0x7f800000u ? 0.f : x - __uint_as_float(bits);
+          };
+          __nv_bfloat16* const dst = a.h + (long long)(off + j) * a.F + row / 2;
+          *reinterpret_cast<uint32_t*>(dst) = hi;
+          *reinterpret_cast<uint32_t*>(dst + (long long)a.slots * a.F) =
+              pack_bf16x2(rest(h, hi << 16), rest(next, hi & 0xffff0000u));
+        }
       };
       if constexpr (UP) {
         if (whole) {
@@ -409,10 +531,17 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           asm volatile("bar.sync 1, 128;" ::: "memory");
           if (sm.last) {
             __threadfence();
-            for (int j = 0; j < n; j++) {
-              float v = 0.f;
-              for (int c = c0; c <= c1; c++) v += __ldcg(tile(c) + (long long)j * BM);
-              swiglu(j, v);
+            constexpr int COLS = 4;  // columns in flight
+            for (int j0 = 0; j0 < n; j0 += COLS) {
+              float v[COLS] = {};
+              for (int c = c0; c <= c1; c++) {
+                const float* const from = tile(c);
+#pragma unroll
+                for (int u = 0; u < COLS; u++) v[u] += __ldcg(from + (long long)min(j0 + u, n - 1) * BM);
+              }
+#pragma unroll
+              for (int u = 0; u < COLS; u++)
+                if (j0 + u < n) swiglu(j0 + u, v[u]);
             }
           }
         }
@@ -438,15 +567,17 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   }
 }
 
-__global__ void __launch_bounds__(128) moe_combine_kernel(Args a, int grid) {
+__global__ void __launch_bounds__(128) moe_combine_kernel(const __grid_constant__ Args a, int grid) {
   const int t = blockIdx.y, d = (blockIdx.x * 128 + threadIdx.x) * 2;
+  pdl_wait();
+  pdl_launch();
   if (d >= a.D) return;
   const Stream st(a.place[a.slots], (a.D + BM - 1) / BM, (a.F + BK - 1) / BK, grid);
   float s0 = 0.f, s1 = 0.f;
   for (int k = 0; k < a.topk; k++) {
     const int at = a.place[t * a.topk + k], slot = at & 0xffff;
     const float w = a.wts[t * a.topk + k];
-    const long long item = (long long)(at >> 16) * st.rt + d / BM;
+    const int item = (at >> 16) * st.rt + d / BM;
     const int n = st.owner((item + 1) * st.kc - 1) - st.owner(item * st.kc) + 1;
     float y0 = 0.f, y1 = 0.f;
     for (int c = 0; c < n; c++) {
@@ -469,7 +600,7 @@ __global__ void __launch_bounds__(128) moe_combine_kernel(Args a, int grid) {
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct Layout {
-  size_t ids, wts, place, done, h, part, y, bytes;
+  size_t logits, wts, place, done, h, part, y, bytes;
   int n_done;
 };
 
@@ -491,24 +622,27 @@ Layout layout_of(const MoeDecodeProblem& p) {
     at += up256(n);
     return r;
   };
-  l.ids = take(slots * 4);
+  l.logits = take((size_t)p.T * p.E * 4);
   l.wts = take(slots * 4);
   l.place = take((slots + 1) * 4);
   l.done = take((size_t)l.n_done * 4);
-  l.h = take(slots * p.F * 2);
+  l.h = take(2 * slots * p.F * 2);
   l.part = take((size_t)p.num_sms * 2 * cols * BM * 4);
   l.y = take((size_t)max_splits(p) * slots * p.D * 4);
   l.bytes = at;
   return l;
 }
 
+// N = 1: the experts' weights lie at equal distances and one map covers them all
 template <int N>
-bool weight_maps(Maps<N>& m, const __nv_bfloat16* const* w, int E, int inner, int rows, long long ld, bool one) {
-  if (one)
+bool weight_maps(Maps<N>& m, const __nv_bfloat16* const* w, int E, int inner, int rows, long long ld) {
+  if constexpr (N == 1) {
     return make_tmap_3d_bf16(&m.w[0], w[0], inner, rows, E, ld, E > 1 ? w[1] - w[0] : 0, BK, BM);
-  for (int e = 0; e < E; e++)
-    if (!make_tmap_3d_bf16(&m.w[e], w[e], inner, rows, 1, ld, 0, BK, BM)) return false;
-  return true;
+  } else {
+    for (int e = 0; e < E; e++)
+      if (!make_tmap_3d_bf16(&m.w[e], w[e], inner, rows, 1, ld, 0, BK, BM)) return false;
+    return true;
+  }
 }
 
 // one tensor map serves all experts when their weights lie at equal distances
@@ -521,38 +655,55 @@ bool evenly_spaced(const __nv_bfloat16* const* w, int E) {
   return true;
 }
 
+template <class... P, class... A>
+cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <bool UP, int N>
 cudaError_t launch_product(const MoeDecodeProblem& p, Args a, cudaStream_t stream) {
   const int inner = UP ? p.D : p.F, rows = UP ? 2 * p.F : p.D;
   const __nv_bfloat16* const* w = UP ? p.w_gate_up : p.w_down;
   Maps<N> maps;
-  a.one_map = evenly_spaced(w, p.E);
-  if (!weight_maps<N>(maps, w, p.E, inner, rows, UP ? p.ld_gate_up : p.ld_down, a.one_map)) return cudaErrorInvalidValue;
-  CUtensorMap tm_b;
-  const bool ok = UP ? make_tmap_2d_bf16_swz(&tm_b, p.x, inner, p.T, p.ldx, BK, a.cols, 128)
-                     : make_tmap_2d_bf16_swz(&tm_b, a.h, inner, a.slots, p.F, BK, a.cols, 128);
+  a.one_map = N == 1;
+  if (!weight_maps<N>(maps, w, p.E, inner, rows, UP ? p.ld_gate_up : p.ld_down)) return cudaErrorInvalidValue;
+  CUtensorMap tm_b, tm_lo;
+  bool ok;
+  if (UP) {
+    ok = make_tmap_2d_bf16_swz(&tm_b, p.x, inner, p.T, p.ldx, BK, a.cols, 128);
+    tm_lo = tm_b;
+  } else {
+    ok = make_tmap_2d_bf16_swz(&tm_b, a.h, inner, a.slots, p.F, BK, 16, 128) &&
+         make_tmap_2d_bf16_swz(&tm_lo, a.h + (size_t)a.slots * p.F, inner, a.slots, p.F, BK, 16, 128);
+  }
   if (!ok) return cudaErrorInvalidValue;
-  const int smem = a.stages * a.stage_bytes + 1024;
+  const int smem = RING_BUDGET + 1024;
   static bool attr = false;
   if (!attr) {
     const cudaError_t e =
-        cudaFuncSetAttribute(moe_product_kernel<UP, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING_BUDGET + 1024);
+        cudaFuncSetAttribute(moe_product_kernel<UP, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     attr = true;
   }
-  moe_product_kernel<UP, N><<<p.num_sms, NTHREADS, smem, stream>>>(tm_b, maps, a);
-  return cudaGetLastError();
+  return launch_overlapped(moe_product_kernel<UP, N>, dim3((unsigned)p.num_sms), NTHREADS, smem, stream, tm_b, tm_lo, maps, a);
 }
 
-template <int N>
-cudaError_t launch_all(const MoeDecodeProblem& p, const Args& a, cudaStream_t stream) {
-  moe_route_kernel<<<p.T, 32 * ROUTE_WARPS, 0, stream>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) e = launch_product<true, N>(p, a, stream);
-  if (e == cudaSuccess) e = launch_product<false, N>(p, a, stream);
-  if (e != cudaSuccess) return e;
-  moe_combine_kernel<<<dim3((p.D + 255) / 256, p.T), 128, 0, stream>>>(a, p.num_sms);
-  return cudaGetLastError();
+template <bool UP>
+cudaError_t launch_product_for(const MoeDecodeProblem& p, const Args& a, cudaStream_t stream) {
+  if (evenly_spaced(UP ? p.w_gate_up : p.w_down, p.E)) return launch_product<UP, 1>(p, a, stream);
+  if (p.E <= 8) return launch_product<UP, 8>(p, a, stream);
+  if (p.E <= 32) return launch_product<UP, 32>(p, a, stream);
+  return launch_product<UP, MAX_E>(p, a, stream);
 }
 
 }  // namespace
@@ -564,6 +715,10 @@ cudaError_t moe_decode(const MoeDecodeProblem& p, cudaStream_t stream) {
   if (p.T > MAX_T || p.E < 1 || p.E > MAX_E || p.topk < 1 || p.topk > MAX_K || p.topk > p.E || p.D < 8 || p.F < 8 ||
       p.D % 8 || p.F % 8 || p.workspace == nullptr)
     return cudaErrorInvalidValue;
+  // tiles are numbered in 32 bits
+  const long long tiles = (long long)p.E * std::max(((2 * p.F + BM - 1) / BM) * (long long)((p.D + BK - 1) / BK),
+                                                    ((p.D + BM - 1) / BM) * (long long)((p.F + BK - 1) / BK));
+  if (tiles > 0x7fffffffLL) return cudaErrorInvalidValue;
   const Layout l = layout_of(p);
   uint8_t* const ws = static_cast<uint8_t*>(p.workspace);
   Args a;
@@ -581,7 +736,7 @@ cudaError_t moe_decode(const MoeDecodeProblem& p, cudaStream_t stream) {
   a.ldres = p.ldres;
   a.out = p.out;
   a.ldo = p.ldo;
-  a.ids = reinterpret_cast<int*>(ws + l.ids);
+  a.logits = reinterpret_cast<float*>(ws + l.logits);
   a.wts = reinterpret_cast<float*>(ws + l.wts);
   a.place = reinterpret_cast<int*>(ws + l.place);
   a.done = reinterpret_cast<unsigned int*>(ws + l.done);
@@ -590,12 +745,12 @@ cudaError_t moe_decode(const MoeDecodeProblem& p, cudaStream_t stream) {
   a.part = reinterpret_cast<float*>(ws + l.part);
   a.y = reinterpret_cast<float*>(ws + l.y);
   a.cols = (p.T + 15) / 16 * 16;
-  a.stage_bytes = A_BYTES + a.cols * BK * 2;
-  a.stages = std::min(MAX_STAGES, RING_BUDGET / a.stage_bytes);
-  a.one_map = 0;
-  if (p.E <= 8) return launch_all<8>(p, a, stream);
-  if (p.E <= 32) return launch_all<32>(p, a, stream);
-  return launch_all<MAX_E>(p, a, stream);
+  cudaError_t e = launch_overlapped(moe_logits_kernel, dim3((unsigned)p.E, (unsigned)((p.T + LOGIT_TOKENS - 1) / LOGIT_TOKENS)),
+                                    32 * LOGIT_WARPS, 0, stream, a);
+  if (e == cudaSuccess) e = launch_product_for<true>(p, a, stream);
+  if (e == cudaSuccess) e = launch_product_for<false>(p, a, stream);
+  if (e != cudaSuccess) return e;
+  return launch_overlapped(moe_combine_kernel, dim3((unsigned)((p.D + 255) / 256), (unsigned)p.T), 128, 0, stream, a, p.num_sms);
 }
 
 }  // namespace ft
