@@ -138,8 +138,8 @@ __global__ void __launch_bounds__(32 * LOGIT_WARPS) moe_logits_kernel(const __gr
 
 // A token's experts by repeated maximum, by a whole warp: equal logits go to the lower expert, NaN
 // counts as the largest. Lane k < topk gets choice k and its weight.
+template <int PER>  // experts a lane
 __device__ __forceinline__ void choose(const Args& a, int t, int lane, int& mine_e, float& mine_w) {
-  constexpr int PER = MAX_E / 32;
   float v[PER];
   uint32_t key[PER];
 #pragma unroll
@@ -179,11 +179,12 @@ __device__ __forceinline__ void choose(const Args& a, int t, int lane, int& mine
 
 // ------------------------------------------------------------------------------------ the products
 struct Tables {
-  short id[MAX_SLOTS];        // expert of each (token, choice) pair
+  alignas(16) short id[MAX_SLOTS];  // expert of each (token, choice) pair
   short pair[MAX_SLOTS];      // pairs ordered by expert, then token
   short token[MAX_SLOTS];     // and their tokens
   short off[MAX_E + 1];       // first slot of each expert
   short act[MAX_E];           // the experts that were chosen
+  unsigned int used[MAX_E / 32];
   int n_act;
   int most;                   // tokens of the expert with the most
 };
@@ -210,67 +211,66 @@ struct Stream {
 // expert tables of every CTA, from the logits
 __device__ void build_tables(Tables& tb, const Args& a, bool keep_weights) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) tb.most = 0;
   for (int t = warp; t < a.T; t += NTHREADS / 32) {
     int e;
     float w;
-    choose(a, t, lane, e, w);
+    if (a.E <= 32) choose<1>(a, t, lane, e, w);
+    else choose<MAX_E / 32>(a, t, lane, e, w);
     if (lane < a.topk) {
       tb.id[t * a.topk + lane] = (short)e;
       if (keep_weights) a.wts[t * a.topk + lane] = w;
     }
   }
+  if (threadIdx.x < 16 && a.slots + threadIdx.x < MAX_SLOTS) tb.id[a.slots + threadIdx.x] = MAX_E;  // no expert
   __syncthreads();
-  for (int e = warp; e < a.E; e += NTHREADS / 32) {
-    int n = 0;
-    for (int i = 0; i < a.slots; i += 32) n += __popc(__ballot_sync(0xffffffffu, i + lane < a.slots && tb.id[i + lane] == e));
-    if (lane == 0) tb.off[e + 1] = (short)n;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    constexpr int PER = MAX_E / 32;
-    int n[PER], sum = 0, used = 0, most = 0;
+  // a pair's slot is the number of pairs with a lower expert, or the same one and an earlier place
+  for (int i = threadIdx.x; i < a.slots; i += NTHREADS) {
+    const int e = tb.id[i];
+    int at = 0;
+    for (int j0 = 0; j0 < a.slots; j0 += 8) {
+      const uint4 v = *reinterpret_cast<const uint4*>(tb.id + j0);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int e = lane * PER + i;
-      n[i] = e < a.E ? tb.off[e + 1] : 0;
-      sum += n[i];
-      used += n[i] > 0;
-      most = max(most, n[i]);
-    }
-    int s = sum, u = used;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int sv = __shfl_up_sync(0xffffffffu, s, o), uv = __shfl_up_sync(0xffffffffu, u, o);
-      if (lane >= o) s += sv, u += uv;
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 31) tb.n_act = u, tb.most = most;
-    if (lane == 0) tb.off[0] = 0;
-    s -= sum;
-    u -= used;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int e = lane * PER + i;
-      if (e >= a.E) break;
-      s += n[i];
-      if (n[i] > 0) tb.act[u++] = (short)e;
-      tb.off[e + 1] = (short)s;
-    }
-  }
-  __syncthreads();
-  for (int e = warp; e < a.E; e += NTHREADS / 32) {
-    int at = tb.off[e];
-    if (at == tb.off[e + 1]) continue;
-    for (int i = 0; i < a.slots; i += 32) {
-      const bool hit = i + lane < a.slots && tb.id[i + lane] == e;
-      const unsigned int m = __ballot_sync(0xffffffffu, hit);
-      if (hit) {
-        const int to = at + __popc(m & ((1u << lane) - 1));
-        tb.pair[to] = (short)(i + lane);
-        tb.token[to] = (short)((i + lane) / a.topk);
+      for (int k = 0; k < 8; k++) {
+        const int o = (int)(w[k / 2] >> (16 * (k & 1))) & 0xffff;
+        at += o < e || (o == e && j0 + k < i);
       }
-      at += __popc(m);
     }
+    tb.pair[at] = (short)i;
+    tb.token[at] = (short)(i / a.topk);
+  }
+  for (int e0 = 0; e0 < a.E; e0 += NTHREADS) {
+    const int e = e0 + threadIdx.x;
+    int less = 0, same = 0;
+    if (e < a.E) {
+      for (int j0 = 0; j0 < a.slots; j0 += 8) {
+        const uint4 v = *reinterpret_cast<const uint4*>(tb.id + j0);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const int o = (int)(w[k / 2] >> (16 * (k & 1))) & 0xffff;
+          less += o < e;
+          same += o == e;
+        }
+      }
+      tb.off[e] = (short)less;
+      if (e == a.E - 1) tb.off[a.E] = (short)a.slots;
+    }
+    const unsigned int m = __ballot_sync(0xffffffffu, same > 0);
+    const int most = __reduce_max_sync(0xffffffffu, same);
+    if (lane == 0 && e / 32 < MAX_E / 32) {
+      tb.used[e / 32] = m;
+      atomicMax(&tb.most, most);
+    }
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.E; e += NTHREADS) {
+    int at = __popc(tb.used[e / 32] & ((1u << (e % 32)) - 1));
+    for (int i = 0; i < e / 32; i++) at += __popc(tb.used[i]);
+    const bool here = tb.used[e / 32] >> (e % 32) & 1;
+    if (here) tb.act[at] = (short)e;
+    if (e == a.E - 1) tb.n_act = at + here;
   }
   __syncthreads();
 }
@@ -334,8 +334,12 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   const int begin = cta < st.ctas ? st.begin(cta) : 0, end = cta < st.ctas ? st.begin(cta + 1) : 0;
 
   if (UP && cta == 0) {  // where each pair's row of h and of the partial sums is, for the combine kernel
-    for (int ai = warp; ai < tb.n_act; ai += NTHREADS / 32)
-      for (int s = tb.off[tb.act[ai]] + lane; s < tb.off[tb.act[ai] + 1]; s += 32) a.place[tb.pair[s]] = s | ai << 16;
+    for (int s = threadIdx.x; s < a.slots; s += NTHREADS) {
+      const int e = tb.id[tb.pair[s]];
+      int ai = 0;  // its place among the chosen experts
+      while (tb.act[ai] != e) ai++;
+      a.place[tb.pair[s]] = s | ai << 16;
+    }
     if (threadIdx.x == 0) a.place[a.slots] = tb.n_act;
   }
 
@@ -499,6 +503,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
             if (j0 + u < n) use(j0 + u, __uint_as_float(v[u]));
         }
       };
+      auto release = [&]() {  // the accumulator may be written again
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.tempty[acc]);
+      };
       // gate row and up row are neighbouring lanes; four lanes give two outputs of one store
       auto swiglu = [&](int j, float v) {
         const float up = __shfl_down_sync(0xffffffffu, v, 1);
@@ -518,6 +527,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
       if constexpr (UP) {
         if (whole) {
           columns(swiglu);
+          release();
         } else {
           const int c0 = st.owner(item * st.kc), c1 = st.owner((item + 1) * st.kc - 1);
           auto tile = [&](int c) {  // a CTA's run cuts at most two tiles: its first and its last
@@ -525,12 +535,15 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           };
           float* const mine = tile(cta);
           columns([&](int j, float v) { __stcg(mine + (long long)j * BM, v); });
-          __threadfence();
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          if (threadIdx.x == 64) sm.last = atomicAdd(a.done + item, 1u) == (unsigned)(c1 - c0);
+          release();
+          asm volatile("bar.sync 1, 128;" ::: "memory");  // with the fence: every thread's part is there before the count
+          if (threadIdx.x == 64) {
+            __threadfence();
+            sm.last = atomicAdd(a.done + item, 1u) == (unsigned)(c1 - c0);
+            __threadfence();
+          }
           asm volatile("bar.sync 1, 128;" ::: "memory");
           if (sm.last) {
-            __threadfence();
             constexpr int COLS = 4;  // columns in flight
             for (int j0 = 0; j0 < n; j0 += COLS) {
               float v[COLS] = {};
@@ -550,10 +563,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         columns([&](int j, float v) {
           if (row < rows) __stcg(dst + (long long)j * a.D, v);
         });
+        release();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.tempty[acc]);
       acc ^= 1;
       if (acc == 0) acc_ph ^= 1;
       i = stop;
@@ -572,21 +583,41 @@ __global__ void __launch_bounds__(128) moe_combine_kernel(const __grid_constant_
   pdl_wait();
   pdl_launch();
   if (d >= a.D) return;
-  const Stream st(a.place[a.slots], (a.D + BM - 1) / BM, (a.F + BK - 1) / BK, grid);
+  // every load of the choices before the first use, then the first two partial sums of each
+  int at[MAX_K], n[MAX_K];
+  float w[MAX_K];
+  float2 v[MAX_K], u[MAX_K];
+#pragma unroll
+  for (int k = 0; k < MAX_K; k++) {
+    const int i = t * a.topk + min(k, a.topk - 1);
+    at[k] = __ldcg(a.place + i);
+    w[k] = __ldcg(a.wts + i);
+  }
+  const Stream st(__ldcg(a.place + a.slots), (a.D + BM - 1) / BM, (a.F + BK - 1) / BK, grid);
+  const float* const y = a.y + d;
+  const long long part = (long long)a.slots * a.D;
+#pragma unroll
+  for (int k = 0; k < MAX_K; k++) {
+    if (k >= a.topk) break;
+    const int item = (at[k] >> 16) * st.rt + d / BM;
+    n[k] = st.owner((item + 1) * st.kc - 1) - st.owner(item * st.kc) + 1;
+    at[k] &= 0xffff;
+    v[k] = __ldcg(reinterpret_cast<const float2*>(y + (long long)at[k] * a.D));
+    u[k] = make_float2(0.f, 0.f);
+    if (n[k] > 1) u[k] = __ldcg(reinterpret_cast<const float2*>(y + part + (long long)at[k] * a.D));
+  }
   float s0 = 0.f, s1 = 0.f;
-  for (int k = 0; k < a.topk; k++) {
-    const int at = a.place[t * a.topk + k], slot = at & 0xffff;
-    const float w = a.wts[t * a.topk + k];
-    const int item = (at >> 16) * st.rt + d / BM;
-    const int n = st.owner((item + 1) * st.kc - 1) - st.owner(item * st.kc) + 1;
-    float y0 = 0.f, y1 = 0.f;
-    for (int c = 0; c < n; c++) {
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(a.y + ((long long)c * a.slots + slot) * a.D + d));
-      y0 += v.x;
-      y1 += v.y;
+#pragma unroll
+  for (int k = 0; k < MAX_K; k++) {
+    if (k >= a.topk) break;
+    float y0 = v[k].x + u[k].x, y1 = v[k].y + u[k].y;
+    for (int c = 2; c < n[k]; c++) {
+      const float2 x = __ldcg(reinterpret_cast<const float2*>(y + c * part + (long long)at[k] * a.D));
+      y0 += x.x;
+      y1 += x.y;
     }
-    s0 = fmaf(w, y0, s0);
-    s1 = fmaf(w, y1, s1);
+    s0 = fmaf(w[k], y0, s0);
+    s1 = fmaf(w[k], y1, s1);
   }
   if (a.residual) {
     const uint32_t r = *reinterpret_cast<const uint32_t*>(a.residual + t * a.ldres + d);
