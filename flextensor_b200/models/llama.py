@@ -23,6 +23,8 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from flextensor_b200.models.kv_cache import QuantizedKV, attend, check_draft, new_layer_cache, store
+
 
 @dataclass
 class LlamaConfig:
@@ -94,9 +96,11 @@ class LlamaLayer(nn.Module):
     def attention_fused(self, x, B, S, rope, cache=None, pos: int = 0):
         """x += o_proj(causal GQA attention(RMSNorm(x))), native kernels, in place.
 
-        ``cache`` = (k_cache, v_cache) ``[B, L_max, Hk, 128]``: prefill (``pos == 0``, S tokens)
+        ``cache`` = (k_cache, v_cache) ``[B, L_max, Hk, 128]`` or an 8-bit
+        :class:`~flextensor_b200.models.kv_cache.QuantizedKV`: prefill (``pos == 0``, S tokens)
         stores the rotated keys and the values of positions [0, S); a decode step (S == 1,
-        ``rope`` holding position ``pos``) appends position ``pos`` and attends over [0, pos]."""
+        ``rope`` holding position ``pos``) appends position ``pos`` and attends over [0, pos]. On an
+        8-bit cache a step may hold several tokens (``pos > 0``, ``rope`` from ``pos`` on)."""
         from flextensor_b200 import ops
 
         cfg, D = self.cfg, self.cfg.head_dim
@@ -110,11 +114,9 @@ class LlamaLayer(nn.Module):
         if cache is None:
             o = ops.attention(qv, kv_, vv, causal=True)
         else:
-            kc, vc = cache
-            kc[:, pos:pos + S].copy_(kv_)
-            vc[:, pos:pos + S].copy_(vv)
-            if S == 1:  # decode: one query per sequence over the cached keys [0, pos]
-                o = ops.decode_attention(qv, kc, vc, pos + 1)
+            store(cache, kv_, vv, pos)
+            if S == 1 or (pos > 0 and isinstance(cache, QuantizedKV)):  # decode: the new tokens' queries over the cached keys
+                o = attend(cache, qv, pos + S)
             else:
                 o = ops.attention(qv, kv_, vv, causal=True)
         ops.linear(o.reshape(B * S, -1), self.wo, None, epi="res", residual=x, out=x)
@@ -178,11 +180,9 @@ class LlamaLayer(nn.Module):
         ops.rope(k, *rope, D, S, out=k)
         qv, kv_, vv = q.view(B, S, self.hq, D), k.view(B, S, self.hk, D), v.view(B, S, self.hk, D)
         if cache is not None:
-            kc, vc = cache
-            kc[:, pos:pos + S].copy_(kv_)
-            vc[:, pos:pos + S].copy_(vv)
-        if cache is not None and S == 1:
-            o = ops.decode_attention(qv, cache[0], cache[1], pos + 1)
+            store(cache, kv_, vv, pos)
+        if cache is not None and (S == 1 or (pos > 0 and isinstance(cache, QuantizedKV))):
+            o = attend(cache, qv, pos + S)
         else:
             o = ops.attention(qv, kv_, vv, causal=True)
         scattered_gemm(o.view(B * S, -1), self.wo)
@@ -230,11 +230,11 @@ class LlamaModel(nn.Module):
 
     # ---------------------------------------------------------------- KV-cache generation
     def new_cache(self, batch: int, max_len: int, device=None, dtype=torch.bfloat16):
+        """One cache a layer: bf16 pairs, or with ``dtype`` ``torch.int8`` / ``torch.float8_e4m3fn`` 8-bit
+        codes with a scale per block of tokens and head."""
         cfg = self.cfg
         dev = device or self.lm_head.device
-        return [(torch.empty(batch, max_len, cfg.n_kv_heads, cfg.head_dim, device=dev, dtype=dtype),
-                 torch.empty(batch, max_len, cfg.n_kv_heads, cfg.head_dim, device=dev, dtype=dtype))
-                for _ in self.layers]
+        return [new_layer_cache(batch, max_len, cfg.n_kv_heads, cfg.head_dim, dev, dtype) for _ in self.layers]
 
     def _logits(self, h_last):
         return F.linear(_rms_torch(h_last, self.norm, self.cfg.eps), self.lm_head)
@@ -252,20 +252,24 @@ class LlamaModel(nn.Module):
 
     @torch.no_grad()
     def decode_step(self, token: torch.Tensor, cache, pos: int) -> torch.Tensor:
-        """One new token per sequence at position ``pos``; returns its logits ``[B, vocab]``."""
+        """One new token per sequence at position ``pos``; returns its logits ``[B, vocab]``. On an 8-bit
+        cache ``token`` may be ``[B, S]``, S > 1, the tokens of positions ``[pos, pos + S)`` (a draft to
+        check); the logits are then ``[B, S, vocab]``."""
         B = token.shape[0]
-        x = self.embed(token.view(B)).contiguous()
+        S = check_draft(token, cache)
+        x = self.embed(token.reshape(B * S)).contiguous()
         cos, sin = self.rope(cache[0][0].shape[1], x.device)
-        rope_p = (cos[pos:pos + 1].contiguous(), sin[pos:pos + 1].contiguous())
+        rope_p = (cos[pos:pos + S].contiguous(), sin[pos:pos + S].contiguous())
         for layer, c in zip(self.layers, cache):
-            x = layer(x, B, 1, rope_p, self.impl, cache=c, pos=pos)
-        return self._logits(x)
+            x = layer(x, B, S, rope_p, self.impl, cache=c, pos=pos)
+        logits = self._logits(x)
+        return logits if S == 1 else logits.view(B, S, -1)
 
     @torch.no_grad()
-    def generate(self, tokens: torch.Tensor, max_new: int) -> torch.Tensor:
-        """Greedy continuation ``[B, max_new]`` with a KV cache."""
+    def generate(self, tokens: torch.Tensor, max_new: int, cache_dtype=torch.bfloat16) -> torch.Tensor:
+        """Greedy continuation ``[B, max_new]`` with a KV cache of ``cache_dtype``."""
         B, S = tokens.shape
-        cache = self.new_cache(B, S + max_new, tokens.device)
+        cache = self.new_cache(B, S + max_new, tokens.device, cache_dtype)
         logits = self.prefill(tokens, cache)
         out = []
         for i in range(max_new):
@@ -365,12 +369,11 @@ class LlamaTP(nn.Module):
         self._ag = self._rs = None
 
     def new_cache(self, batch: int, max_len: int, device=None, dtype=torch.bfloat16):
-        """This rank's KV cache: its ``n_kv_heads / world`` heads of every layer."""
-        D = self.cfg.head_dim
-        hk = self.cfg.n_kv_heads // self.world
+        """This rank's KV cache: its ``n_kv_heads / world`` heads of every layer (``dtype`` as in
+        :meth:`LlamaModel.new_cache`)."""
         dev = device or torch.device("cuda", torch.cuda.current_device())
-        return [(torch.empty(batch, max_len, hk, D, device=dev, dtype=dtype),
-                 torch.empty(batch, max_len, hk, D, device=dev, dtype=dtype)) for _ in self.layers]
+        return [new_layer_cache(batch, max_len, self.cfg.n_kv_heads // self.world, self.cfg.head_dim, dev, dtype)
+                for _ in self.layers]
 
     def forward(self, x_local: torch.Tensor, B: int, S: int, rope, cache=None, pos: int = 0) -> torch.Tensor:
         """x_local ``[B*S/world, dim]`` (this rank's token rows) -> same rows after all layers.

@@ -4,9 +4,11 @@ Attention is the Llama block (``models/llama.py``, native kernels). The MoE feed
 router logits -> top-2 -> softmax over the two; each expert is a SwiGLU FFN whose gate/up
 rows are interleaved (one GEMM with the SwiGLU epilogue) followed by the down GEMM.
 
-Three MoE paths share one parameter tree:
+Four MoE paths share one parameter tree:
 
 * single GPU (``ep=None``): per-expert gather -> fused GEMMs -> weighted scatter-add;
+* single GPU, few tokens (``MixtralConfig.moe_decode``): the whole layer in one call without host
+  synchronisation (``ops.moe_decode``);
 * expert parallel, fused (``ep=ExpertParallel``): each rank keeps its own tokens and owns
   ``E/world`` experts; dispatch / combine run inside the expert GEMM kernels over NVLink
   (``parallel/ep.py``, ``ops/csrc/moe_sm100.cu``);
@@ -25,6 +27,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from flextensor_b200.models.kv_cache import check_draft, new_layer_cache
 from flextensor_b200.models.llama import LlamaConfig, LlamaLayer, _rms_torch, rope_tables_1d
 
 
@@ -39,6 +42,7 @@ class MixtralConfig(LlamaConfig):
     rope_theta: float = 1000000.0
     n_experts: int = 8
     topk: int = 2
+    moe_decode: bool = False  # single GPU, native path: steps of at most 64 tokens take ops.moe_decode
 
 
 MIXTRAL_8X22B = MixtralConfig()
@@ -101,6 +105,10 @@ class MixtralLayer(nn.Module):
         else:
             x = self.attn.attention_torch(x, B, S, rope)
         h = ops.rmsnorm(x, self.ffn_norm, eps=cfg.eps) if impl == "fused" else _rms_torch(x, self.ffn_norm, cfg.eps)
+        if (ep is None and impl == "fused" and cfg.moe_decode and h.shape[0] <= ops.MOE_DECODE_MAX_TOKENS
+                and len(self.experts) == cfg.n_experts):
+            return ops.moe_decode(h, self.router, [e.w_gate_up for e in self.experts],
+                                  [e.w_down for e in self.experts], cfg.topk, residual=x, out=x)
         ids, wts = route_topk(h, self.router, cfg.topk)
         if ep is None:
             return self.moe_single(h, ids, wts, x, impl)
@@ -146,11 +154,10 @@ class MixtralModel(nn.Module):
 
     # ---------------------------------------------------------------- KV-cache generation
     def new_cache(self, batch: int, max_len: int, device=None, dtype=torch.bfloat16):
+        """One cache a layer, bf16 or 8 bits (``dtype`` ``torch.int8`` / ``torch.float8_e4m3fn``)."""
         cfg = self.cfg
         dev = device or self.lm_head.device
-        return [(torch.empty(batch, max_len, cfg.n_kv_heads, cfg.head_dim, device=dev, dtype=dtype),
-                 torch.empty(batch, max_len, cfg.n_kv_heads, cfg.head_dim, device=dev, dtype=dtype))
-                for _ in self.layers]
+        return [new_layer_cache(batch, max_len, cfg.n_kv_heads, cfg.head_dim, dev, dtype) for _ in self.layers]
 
     def _logits(self, h_last):
         return F.linear(_rms_torch(h_last, self.norm, self.cfg.eps), self.lm_head)
@@ -168,20 +175,23 @@ class MixtralModel(nn.Module):
 
     @torch.no_grad()
     def decode_step(self, token: torch.Tensor, cache, pos: int, ep=None) -> torch.Tensor:
-        """One new token per sequence at position ``pos``; returns its logits ``[B, vocab]``."""
+        """One new token per sequence at position ``pos``; returns its logits ``[B, vocab]``. On an 8-bit
+        cache ``token`` may be ``[B, S]``, S > 1 (a draft to check); the logits are then ``[B, S, vocab]``."""
         B = token.shape[0]
-        x = self.embed(token.view(B)).contiguous()
+        S = check_draft(token, cache)
+        x = self.embed(token.reshape(B * S)).contiguous()
         cos, sin = self.rope(cache[0][0].shape[1], x.device)
-        rope_p = (cos[pos:pos + 1].contiguous(), sin[pos:pos + 1].contiguous())
+        rope_p = (cos[pos:pos + S].contiguous(), sin[pos:pos + S].contiguous())
         for layer, c in zip(self.layers, cache):
-            x = layer(x, B, 1, rope_p, self.impl, ep=ep, cache=c, pos=pos)
-        return self._logits(x)
+            x = layer(x, B, S, rope_p, self.impl, ep=ep, cache=c, pos=pos)
+        logits = self._logits(x)
+        return logits if S == 1 else logits.view(B, S, -1)
 
     @torch.no_grad()
-    def generate(self, tokens: torch.Tensor, max_new: int, ep=None) -> torch.Tensor:
-        """Greedy continuation ``[B, max_new]`` with a KV cache."""
+    def generate(self, tokens: torch.Tensor, max_new: int, ep=None, cache_dtype=torch.bfloat16) -> torch.Tensor:
+        """Greedy continuation ``[B, max_new]`` with a KV cache of ``cache_dtype``."""
         B, S = tokens.shape
-        cache = self.new_cache(B, S + max_new, tokens.device)
+        cache = self.new_cache(B, S + max_new, tokens.device, cache_dtype)
         logits = self.prefill(tokens, cache, ep)
         out = []
         for i in range(max_new):
@@ -207,9 +217,7 @@ class MixtralStack(nn.Module):
     def new_cache(self, batch: int, max_len: int, device=None, dtype=torch.bfloat16):
         c = self.cfg
         dev = device or torch.device("cuda", torch.cuda.current_device())
-        return [(torch.empty(batch, max_len, c.n_kv_heads, c.head_dim, device=dev, dtype=dtype),
-                 torch.empty(batch, max_len, c.n_kv_heads, c.head_dim, device=dev, dtype=dtype))
-                for _ in self.layers]
+        return [new_layer_cache(batch, max_len, c.n_kv_heads, c.head_dim, dev, dtype) for _ in self.layers]
 
     def forward(self, x, B, S, rope, ep: dict | None = None, cache=None, pos: int = 0):
         e = None if not ep else ep.get(x.shape[0])
