@@ -304,20 +304,39 @@ struct QueryFrag {
   int row[NT][2];    // rows of those columns
 };
 
+// Their bf16 rows as they lie in memory: 64 bytes a lane and row. Loaded apart from their conversion,
+// so that the loads are on their way before the keys and values that fill the memory's queues.
 template <int NT>
-__device__ __forceinline__ void load_queries(QueryFrag<NT>& f, const DecArgs& a, int b, int h, int row0, int lane) {
+struct RawQueries {
+  uint4 w[NT][4];
+  int row0;
+};
+
+template <int NT>
+__device__ __forceinline__ void load_queries(RawQueries<NT>& raw, const DecArgs& a, int b, int h, int row0, int lane) {
   const int g = lane >> 2, c = lane & 3;
+  raw.row0 = row0;
 #pragma unroll
   for (int nt = 0; nt < NT; nt++) {
     const int r = row0 + nt * 8 + g;
-    uint4 w[4] = {};
-    if (r < a.R) {
-      const uint4* p = reinterpret_cast<const uint4*>(a.q + b * a.q_b + (long long)(r / a.G) * a.q_tok +
-                                                      (long long)(h * a.G + r % a.G) * a.q_h + 32 * c);
+    const uint4* p = reinterpret_cast<const uint4*>(a.q + b * a.q_b + (long long)(r / a.G) * a.q_tok +
+                                                    (long long)(h * a.G + r % a.G) * a.q_h + 32 * c);
 #pragma unroll
-      for (int i = 0; i < 4; i++) w[i] = p[i];
+    for (int i = 0; i < 4; i++) {
+      raw.w[nt][i] = make_uint4(0, 0, 0, 0);
+      if (r < a.R) raw.w[nt][i] = p[i];
     }
-    const uint32_t* x = reinterpret_cast<const uint32_t*>(w);
+  }
+}
+
+template <int NT>
+__device__ __forceinline__ void convert_queries(QueryFrag<NT>& f, const RawQueries<NT>& raw, const DecArgs& a, int lane) {
+  const int c = lane & 3, row0 = raw.row0;
+#pragma unroll
+  for (int nt = 0; nt < NT; nt++) {
+    const uint4(&w)[4] = raw.w[nt];
+    const uint32_t x[16] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w,
+                            w[2].x, w[2].y, w[2].z, w[2].w, w[3].x, w[3].y, w[3].z, w[3].w};
     uint32_t m2 = 0;
 #pragma unroll
     for (int i = 0; i < 16; i++) m2 = __vmaxu2(m2, x[i] & 0x7fff7fffu);
@@ -647,20 +666,17 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
       if (two) tma_load_4d(dst + UNIT_BYTES, map, &full[s], 0, z, (ahead.t + 1) * UNIT, w);
     }
   };
-  fetch(0, false);
-  fetch(1, true);
-  bool more = ahead.next(a, step, start);  // whether `ahead` is a tile after `at`
-  if (more) fetch(2, false);
   QueryFrag<NT> qf;
+  RawQueries<NT> raw;
   RowState<NT> st;
-  int sees[NT][2], len = 0;
+  int sees[NT][2], len = 0, len_next = 0;
   const float *ksp = nullptr, *vsp = nullptr;  // the head's scales
   TileScales<MT> sc;
-  // 16 keys never straddle a block, and a tile of a whole block or less takes one scale; what lies
-  // past the length takes the last block's
-  auto scales = [&](int t) {
+  // The scales of the tile at unit t of a sequence of n keys. 16 keys never straddle a block, and a
+  // tile of a whole block or less takes one scale; what lies past the length takes the last block's.
+  auto scales = [&](int t, int n) {
     if (16 * MT <= 1 << a.block_shift) {
-      const int blk = (t * UNIT) >> a.block_shift, blk2 = min(t * UNIT + 16 * MT - 1, len - 1) >> a.block_shift;
+      const int blk = (t * UNIT) >> a.block_shift, blk2 = min(t * UNIT + 16 * MT - 1, n - 1) >> a.block_shift;
       const float k0 = ksp[(long long)blk * a.k.s_blk], v0 = vsp[(long long)blk * a.v.s_blk];
       const float k1 = ksp[(long long)blk2 * a.k.s_blk], v1 = vsp[(long long)blk2 * a.v.s_blk];
 #pragma unroll
@@ -672,18 +688,22 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
     }
 #pragma unroll
     for (int i = 0; i < MT; i++) {
-      const int blk = min(t * UNIT + 16 * i, len - 1) >> a.block_shift;
+      const int blk = min(t * UNIT + 16 * i, n - 1) >> a.block_shift;
       sc.k[i] = ksp[(long long)blk * a.k.s_blk];
       sc.v[i] = vsp[(long long)blk * a.v.s_blk];
     }
   };
-  auto enter = [&]() {  // a new head: its queries, empty accumulators
-    const int hg = at.j * a.heads + my_head, h = hg / a.n_group;
-    len = seq_len(a, at.b);
-    ksp = a.k.scale + at.b * a.k.s_b + h * a.k.s_h;
-    vsp = a.v.scale + at.b * a.v.s_b + h * a.v.s_h;
-    scales(at.t);
-    load_queries<NT>(qf, a, at.b, h, (hg - h * a.n_group) * 8 * NT, lane);
+  auto prepare = [&](const Cursor& x) {  // the loads for a new head, whose first tile is at x
+    const int hg = x.j * a.heads + my_head, h = hg / a.n_group;
+    len_next = seq_len(a, x.b);
+    ksp = a.k.scale + x.b * a.k.s_b + h * a.k.s_h;
+    vsp = a.v.scale + x.b * a.v.s_b + h * a.v.s_h;
+    load_queries<NT>(raw, a, x.b, h, (hg - h * a.n_group) * 8 * NT, lane);
+    scales(x.t, len_next);
+  };
+  auto enter = [&]() {  // the new head: its queries, empty accumulators
+    len = len_next;
+    convert_queries<NT>(qf, raw, a, lane);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -696,6 +716,11 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
       }
     }
   };
+  prepare(at);  // before the copies: behind 192 KB an SM of them these loads took 5 us
+  fetch(0, false);
+  fetch(1, true);
+  bool more = ahead.next(a, step, start);  // whether `ahead` is a tile after `at`
+  if (more) fetch(2, false);
   enter();
   bool ok = true;
   int s = 0;        // slot of the next piece to read
@@ -735,7 +760,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
       };
       auto values_here = [&]() { return ok = __all_sync(0xffffffffu, bounded_wait(&full[s], ph)); };
       const TileScales<MT> now = sc;
-      if (!last) scales(ahead.t);  // in flight during the tile
+      if (!last) scales(ahead.t, len);  // in flight during the tile
+      else if (more) prepare(ahead);
       attend_tile<NT, MT, FMT>(st, qf, kt, vt, now, lim, masked, lane, keys_read, values_here);
       __syncwarp();
     }
@@ -776,7 +802,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
 // Rows of the output: each row's partial results in the order of runs and warps, `merge_per_row` warps a
 // row (each a contiguous part of them), four dims a lane, eight partials in flight.
 template <int NT>
-__global__ void __launch_bounds__(32 * MERGE_WARPS, 2) cache_merge_kernel(const __grid_constant__ DecArgs a) {
+__global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(const __grid_constant__ DecArgs a) {
   __shared__ float4 so[MERGE_WARPS][32];
   __shared__ float2 sml[MERGE_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -785,57 +811,65 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS, 2) cache_merge_kernel(const 
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float M = -INFINITY, L = 0.f;
   int r = 0, h = 0, b = 0, len = 0;
-  pdl_wait();
-  pdl_launch();
+  // The lengths are there: this kernel starts only after every CTA of the first one has waited for what
+  // was before it.
+  int r0 = 0, lo = 0, hi = 0, f = 0, n = 0, stride = 0;
+  long long base = 0;
+  Runs runs(0, 0);
   if (row < rows) {
     r = row % a.R;
     h = row / a.R % a.Hk;
     b = row / a.R / a.Hk;
     len = seq_len(a, b);
-    const int hg = h * a.n_group + r / (8 * NT), j = hg / a.heads, n = (len + UNIT - 1) / UNIT;
-    const Runs runs(units_before(a, a.B, lane), a.runs);
-    const int f = units_before(a, b, lane) + j * n;
+    const int hg = h * a.n_group + r / (8 * NT), j = hg / a.heads;
+    n = (len + UNIT - 1) / UNIT;
+    runs = Runs(units_before(a, a.B, lane), a.runs);
+    f = units_before(a, b, lane) + j * n;
     if (n > 0) {
-      const int r0 = runs.owner(f), cnt = (runs.owner(f + n - 1) + 1 - r0) * a.keys;
-      const int lo = cnt * part / per, hi = cnt * (part + 1) / per;
+      r0 = runs.owner(f);
+      const int cnt = (runs.owner(f + n - 1) + 1 - r0) * a.keys;
+      lo = cnt * part / per;
+      hi = cnt * (part + 1) / per;
       // partial i: run r0 + i / keys, the warp of this head with key tiles i % keys
-      const long long base = (((long long)b * a.per + j + r0) * WARPS + hg - j * a.heads) * (8 * NT) + r % (8 * NT);
-      const int stride = a.heads * 8 * NT;
-      for (int i0 = lo; i0 < hi; i0 += 8) {
-        float4 v[8];
+      base = (((long long)b * a.per + j + r0) * WARPS + hg - j * a.heads) * (8 * NT) + r % (8 * NT);
+      stride = a.heads * 8 * NT;
+    }
+  }
+  pdl_wait();
+  pdl_launch();
+  for (int i0 = lo; i0 < hi; i0 += 8) {
+    float4 v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++)
-          v[i] = __ldcg(reinterpret_cast<const float4*>(a.part_o + (base + (long long)min(i0 + i, hi - 1) * stride) * HD) + lane);
-        float2 ml = make_float2(-INFINITY, 0.f);
-        const int mine = i0 + lane;
-        if (lane < 8 && mine < hi) {
-          // the warp wrote a partial if the run's part of the head reaches its first tile
-          const int run = r0 + mine / a.keys, from = max(f, runs.begin(run)), to = min(f + n, runs.begin(run + 1));
-          if (from + mine % a.keys * units_of_tile(NT) < to) ml = __ldcg(a.part_ml + base + (long long)mine * stride);
-        }
-        float top = ml.x;
+    for (int i = 0; i < 8; i++)
+      v[i] = __ldcg(reinterpret_cast<const float4*>(a.part_o + (base + (long long)min(i0 + i, hi - 1) * stride) * HD) + lane);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    const int mine = i0 + lane;
+    if (lane < 8 && mine < hi) {
+      // the warp wrote a partial if the run's part of the head reaches its first tile
+      const int run = r0 + mine / a.keys, from = max(f, runs.begin(run)), to = min(f + n, runs.begin(run + 1));
+      if (from + mine % a.keys * units_of_tile(NT) < to) ml = __ldcg(a.part_ml + base + (long long)mine * stride);
+    }
+    float top = ml.x;
 #pragma unroll
-        for (int o = 4; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-        top = __shfl_sync(0xffffffffu, top, 0);
-        const float m_new = max_nan(M, top), ref = m_new == -INFINITY ? 0.f : m_new;
-        const float al = M == -INFINITY ? 0.f : ex2f(M - ref), w = ml.x == -INFINITY ? 0.f : ex2f(ml.x - ref);
-        M = m_new;
-        L *= al;
-        acc.x *= al;
-        acc.y *= al;
-        acc.z *= al;
-        acc.w *= al;
+    for (int o = 4; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = __shfl_sync(0xffffffffu, top, 0);
+    const float m_new = max_nan(M, top), ref = m_new == -INFINITY ? 0.f : m_new;
+    const float al = M == -INFINITY ? 0.f : ex2f(M - ref), w = ml.x == -INFINITY ? 0.f : ex2f(ml.x - ref);
+    M = m_new;
+    L *= al;
+    acc.x *= al;
+    acc.y *= al;
+    acc.z *= al;
+    acc.w *= al;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float wi = __shfl_sync(0xffffffffu, w, i), li = __shfl_sync(0xffffffffu, ml.y, i);
-          if (wi == 0.f) continue;  // nothing was written there, or nothing of it counts
-          L = fmaf(wi, li, L);
-          acc.x = fmaf(wi, v[i].x, acc.x);
-          acc.y = fmaf(wi, v[i].y, acc.y);
-          acc.z = fmaf(wi, v[i].z, acc.z);
-          acc.w = fmaf(wi, v[i].w, acc.w);
-        }
-      }
+    for (int i = 0; i < 8; i++) {
+      const float wi = __shfl_sync(0xffffffffu, w, i), li = __shfl_sync(0xffffffffu, ml.y, i);
+      if (wi == 0.f) continue;  // nothing was written there, or nothing of it counts
+      L = fmaf(wi, li, L);
+      acc.x = fmaf(wi, v[i].x, acc.x);
+      acc.y = fmaf(wi, v[i].y, acc.y);
+      acc.z = fmaf(wi, v[i].z, acc.z);
+      acc.w = fmaf(wi, v[i].w, acc.w);
     }
   }
   if (per > 1) {
