@@ -4,6 +4,8 @@
 // launches on the caller's current CUDA stream; a failed launch raises.
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -289,10 +291,10 @@ void check_cache(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Ten
   TORCH_CHECK(block == 16 || block == 32 || block == 64 || block == 128 || block == 256, op,
               ": block must be 16, 32, 64, 128 or 256 tokens, got ", block);
   TORCH_CHECK(kc.size(1) < (1LL << 30), op, ": the cache is too long");
-  const std::vector<int64_t> want = {kc.size(0), (kc.size(1) + block - 1) / block, kc.size(2)};
-  TORCH_CHECK(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat && ks.sizes() == at::IntArrayRef(want) &&
-                  vs.sizes() == at::IntArrayRef(want),
-              op, ": scales must be fp32 [B, ceil(L / block), Hk] = ", at::IntArrayRef(want), ", got ", ks.sizes(), " and ",
+  const std::array<int64_t, 3> blocks = {kc.size(0), (kc.size(1) + block - 1) / block, kc.size(2)};
+  const at::IntArrayRef want(blocks);
+  TORCH_CHECK(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat && ks.sizes() == want && vs.sizes() == want,
+              op, ": scales must be fp32 [B, ceil(L / block), Hk] = ", want, ", got ", ks.sizes(), " and ",
               vs.sizes());
   for (const Tensor* t : {&kc, &vc}) {
     TORCH_CHECK(t->stride(3) == 1 && t->stride(0) % 16 == 0 && t->stride(1) % 16 == 0 && t->stride(2) % 16 == 0 &&
@@ -315,11 +317,14 @@ ft::CacheSide cache_side(const Tensor& c, const Tensor& s) {
 }
 
 // rows of 128 bf16 values that 16-byte loads can take
-void check_rows(const Tensor& t, const char* op, const char* name) {
+void check_rows(const Tensor& t, const char* op, const char* name, bool may_be_3d = false) {
   TORCH_CHECK(t.scalar_type() == at::kBFloat16, op, ": ", name, " must be bfloat16");
-  TORCH_CHECK(t.dim() == 4 && t.size(3) == kHead, op, ": ", name, " must be [B, S, H, 128], got ", t.sizes());
-  TORCH_CHECK(t.stride(3) == 1 && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(2) % 8 == 0 && on_16_bytes(t),
-              op, ": rows of ", name, " must be contiguous and start on 16-byte boundaries");
+  const int64_t d = t.dim();
+  TORCH_CHECK((d == 4 || (d == 3 && may_be_3d)) && t.size(d - 1) == kHead, op, ": ", name, " must be [B, S, H, 128]",
+              may_be_3d ? " or [B, H, 128]" : "", ", got ", t.sizes());
+  bool aligned = t.stride(d - 1) == 1 && on_16_bytes(t);
+  for (int64_t i = 0; i + 1 < d; i++) aligned = aligned && t.stride(i) % 8 == 0;
+  TORCH_CHECK(aligned, op, ": rows of ", name, " must be contiguous and start on 16-byte boundaries");
 }
 
 void check_lengths(const c10::optional<Tensor>& t, int64_t B, const char* op, const char* name) {
@@ -380,17 +385,18 @@ void kv_append_q8(const Tensor& k, const Tensor& v, Tensor& kc, Tensor& vc, Tens
   check_ok(ft::cache_append(p, at::cuda::getCurrentCUDAStream()), op);
 }
 
-Tensor decode_attention_q8(const Tensor& q_in, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
+Tensor decode_attention_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
                            const c10::optional<Tensor>& o_given, const c10::optional<Tensor>& kv_len, int64_t len_all,
                            int64_t max_len, int64_t block, double scale) {
   const char* op = "decode_attention_q8";
   check_cache(kc, vc, ks, vs, block, op);
-  const Tensor q = q_in.dim() == 3 ? q_in.unsqueeze(1) : q_in;
-  check_rows(q, op, "q");
-  const Tensor o_in = o_given && o_given->defined() ? *o_given : at::empty(q_in.sizes(), q_in.options());
-  const Tensor o = o_in.dim() == 3 ? o_in.unsqueeze(1) : o_in;
-  check_rows(o, op, "out");
-  const int64_t B = kc.size(0), L = kc.size(1), Hk = kc.size(2), Sq = q.size(1), Hq = q.size(2);
+  check_rows(q, op, "q", true);
+  const Tensor o = o_given && o_given->defined() ? *o_given
+                   : q.is_cuda() ? Tensor(at::detail::empty_cuda(q.sizes(), at::kBFloat16, q.device(), c10::nullopt))
+                                 : at::empty_like(q);
+  check_rows(o, op, "out", true);
+  const bool many = q.dim() == 4;
+  const int64_t B = kc.size(0), L = kc.size(1), Hk = kc.size(2), Sq = many ? q.size(1) : 1, Hq = q.size(many ? 2 : 1);
   TORCH_CHECK(q.size(0) == B, op, ": q has ", q.size(0), " sequences, the cache ", B);
   TORCH_CHECK(o.sizes() == q.sizes(), op, ": out must have the shape of q");
   TORCH_CHECK(Hk > 0 && Hq % Hk == 0, op, ": query heads must be a multiple of kv heads, got ", Hq, " and ", Hk);
@@ -411,12 +417,12 @@ Tensor decode_attention_q8(const Tensor& q_in, const Tensor& kc, const Tensor& v
   p.format = kc.scalar_type() == at::kChar ? ft::CACHE_INT8 : ft::CACHE_E4M3;
   p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
   p.q_b = q.stride(0);
-  p.q_tok = q.stride(1);
-  p.q_h = q.stride(2);
+  p.q_tok = many ? q.stride(1) : 0;
+  p.q_h = q.stride(many ? 2 : 1);
   p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
   p.o_b = o.stride(0);
-  p.o_tok = o.stride(1);
-  p.o_h = o.stride(2);
+  p.o_tok = many ? o.stride(1) : 0;
+  p.o_h = o.stride(many ? 2 : 1);
   p.side[0] = cache_side(kc, ks);
   p.side[1] = cache_side(vc, vs);
   p.kv_len = each ? kv_len->data_ptr<int>() : nullptr;
@@ -424,11 +430,11 @@ Tensor decode_attention_q8(const Tensor& q_in, const Tensor& kc, const Tensor& v
   p.max_len = (int)(each ? max_len : len_all);
   p.scale = (float)scale;
   p.num_sms = num_sms_for(kc.get_device());
-  if (q.numel() == 0) return o_in;
-  const Tensor scratch = at::empty({(int64_t)ft::cache_decode_scratch_floats(p)}, ks.options());
-  p.scratch = scratch.data_ptr<float>();
+  if (q.numel() == 0) return o;
+  const auto scratch = c10::cuda::CUDACachingAllocator::get()->allocate(ft::cache_decode_scratch_floats(p) * sizeof(float));
+  p.scratch = static_cast<float*>(scratch.get());
   check_ok(ft::cache_decode(p, at::cuda::getCurrentCUDAStream()), op);
-  return o_in;
+  return o;
 }
 
 Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tensor>& gate_up,
@@ -457,7 +463,9 @@ Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tenso
               ": D and F must be multiples of 8, got ", D, " and ", F);
   matrix(x, "x", T, D);
   matrix(router, "router", E, D);
-  const Tensor out = out_given && out_given->defined() ? *out_given : at::empty({T, D}, x.options());
+  const Tensor out = out_given && out_given->defined() ? *out_given
+                     : x.is_cuda() ? Tensor(at::detail::empty_cuda({T, D}, at::kBFloat16, x.device(), c10::nullopt))
+                                   : at::empty({T, D}, x.options());
   matrix(out, "out", T, D);
   const bool res = residual && residual->defined();
   if (res) matrix(*residual, "residual", T, D);
@@ -500,8 +508,8 @@ Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tenso
   p.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
   p.ldo = out.stride(0);
   p.num_sms = num_sms_for(x.get_device());
-  Tensor ws = at::empty({(int64_t)ft::moe_decode_workspace(p)}, x.options().dtype(at::kByte));
-  p.workspace = ws.data_ptr();
+  const auto workspace = c10::cuda::CUDACachingAllocator::get()->allocate(ft::moe_decode_workspace(p));
+  p.workspace = workspace.get();
   check_ok(ft::moe_decode(p, at::cuda::getCurrentCUDAStream()), op);
   return out;
 }
