@@ -221,6 +221,9 @@ constexpr int SLOTS = 3;     // per warp, keys and values in turn
 // Units of a tile: two column tiles leave registers for one
 constexpr int units_of_tile(int column_tiles) { return column_tiles == 1 ? 2 : 1; }
 constexpr int UNIT_BYTES = UNIT * HD;
+// What entering a head costs a warp (its queries, its partial result, a tile cut short), in units: runs
+// are equal in units plus this much for each head and sequence
+constexpr int ENTRY = 1;
 constexpr int MERGE_WARPS = 16;  // at most
 
 struct DecArgs {
@@ -515,16 +518,22 @@ __device__ __forceinline__ int seq_len(const DecArgs& a, int b) {
 }
 __device__ __forceinline__ int seq_units(const DecArgs& a, int b) { return (seq_len(a, b) + UNIT - 1) / UNIT; }
 
-// sum of the units of sequences [0, end) over all steps of heads, by a whole warp
-__device__ __forceinline__ int units_before(const DecArgs& a, int end, int lane) {
-  if (a.kv_len == nullptr) return end * seq_units(a, 0) * a.per;
+// the length of a sequence's share of the work in one step of heads: ENTRY places for the entry, then its units
+__device__ __forceinline__ int seq_cost(const DecArgs& a, int b) {
+  const int n = seq_units(a, b);
+  return n ? n + ENTRY : 0;
+}
+
+// sum of the costs of sequences [0, end) over all steps of heads, by a whole warp
+__device__ __forceinline__ int cost_before(const DecArgs& a, int end, int lane) {
+  if (a.kv_len == nullptr) return end * seq_cost(a, 0) * a.per;
   int sum = 0;
-  for (int b = lane; b < end; b += 32) sum += seq_units(a, b);
+  for (int b = lane; b < end; b += 32) sum += seq_cost(a, b);
   return __reduce_add_sync(0xffffffffu, sum) * a.per;
 }
 
-// The sequence of units (fewer than 2^30, the host checks) and its division into runs, the first
-// `rem` of them one unit longer.
+// The sequence of places (fewer than 2^30, the host checks) and its division into runs, the first
+// `rem` of them one place longer.
 struct Runs {
   int n, base, rem;
   __device__ __forceinline__ Runs(int total, int most) : n(min(most, total)) {
@@ -541,7 +550,7 @@ struct Runs {
 // A warp's place in its CTA's run: a tile of units [t, min(t + units of a tile, end)) of a piece, the
 // run's part of one step of heads of one sequence.
 struct Cursor {
-  int b, j, t, end, left;  // sequence, step of heads, first unit, end of the piece, units of the run after the piece
+  int b, j, t, end, left;  // sequence, step of heads, first unit, end of the piece, places of the run after the piece
 
   // the tile `step` units further on, `start` units into a piece where that leaves this one; false at the run's end
   __device__ __forceinline__ bool next(const DecArgs& a, int step, int start) {
@@ -550,27 +559,28 @@ struct Cursor {
       if (left == 0) return false;
       int n = 0;
       if (++j == a.per) j = 0, b++;
-      while ((n = seq_units(a, b)) == 0) b++;  // units are left, so a sequence with some follows
-      end = min(n, left);
-      left -= end;
+      while ((n = seq_cost(a, b)) == 0) b++;  // places are left, so a sequence with some follows
+      n = min(n, left);
+      left -= n;
+      end = n - ENTRY;
       t = start;
     }
     return true;
   }
 };
 
-// the place of unit i, the first of a run of `count` units, by a whole warp
+// place i, the first of a run of `count`, by a whole warp
 __device__ __forceinline__ Cursor locate(const DecArgs& a, int i, int count, int lane) {
   Cursor c;
   int n;
   if (a.kv_len == nullptr) {
-    n = seq_units(a, 0);
+    n = seq_cost(a, 0);
     c.b = i / (n * a.per);
     i -= c.b * n * a.per;
   } else {
     int before = 0;
     for (int b0 = 0;; b0 += 32) {  // i lies before the total, so some sequence holds it
-      const int mine = b0 + lane < a.B ? seq_units(a, b0 + lane) : 0;
+      const int mine = b0 + lane < a.B ? seq_cost(a, b0 + lane) : 0;
       int end = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -589,9 +599,10 @@ __device__ __forceinline__ Cursor locate(const DecArgs& a, int i, int count, int
     }
   }
   c.j = i / n;
-  c.t = i - c.j * n;
-  c.end = min(n, c.t + count);
-  c.left = count - (c.end - c.t);
+  i -= c.j * n;
+  c.left = count - (min(n, i + count) - i);
+  c.t = max(0, i - ENTRY);
+  c.end = min(n, i + count) - ENTRY;
   return c;
 }
 
@@ -646,7 +657,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
   __syncwarp();
   pdl_wait();
   pdl_launch();
-  const Runs runs(units_before(a, a.B, lane), a.runs);
+  const Runs runs(cost_before(a, a.B, lane), a.runs);
   const int run = blockIdx.x;
   if (run >= runs.n) return;
   const int first = runs.begin(run), count = runs.begin(run + 1) - first;
@@ -822,9 +833,9 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(const __g
     b = row / a.R / a.Hk;
     len = seq_len(a, b);
     const int hg = h * a.n_group + r / (8 * NT), j = hg / a.heads;
-    n = (len + UNIT - 1) / UNIT;
-    runs = Runs(units_before(a, a.B, lane), a.runs);
-    f = units_before(a, b, lane) + j * n;
+    n = seq_cost(a, b);
+    runs = Runs(cost_before(a, a.B, lane), a.runs);
+    f = cost_before(a, b, lane) + j * n;
     if (n > 0) {
       r0 = runs.owner(f);
       const int cnt = (runs.owner(f + n - 1) + 1 - r0) * a.keys;
@@ -846,8 +857,9 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(const __g
     const int mine = i0 + lane;
     if (lane < 8 && mine < hi) {
       // the warp wrote a partial if the run's part of the head reaches its first tile
-      const int run = r0 + mine / a.keys, from = max(f, runs.begin(run)), to = min(f + n, runs.begin(run + 1));
-      if (from + mine % a.keys * units_of_tile(NT) < to) ml = __ldcg(a.part_ml + base + (long long)mine * stride);
+      const int run = r0 + mine / a.keys, from = max(f, runs.begin(run)) - f, to = min(f + n, runs.begin(run + 1)) - f;
+      if (max(0, from - ENTRY) + mine % a.keys * units_of_tile(NT) < to - ENTRY)
+        ml = __ldcg(a.part_ml + base + (long long)mine * stride);
     }
     float top = ml.x;
 #pragma unroll
@@ -1005,8 +1017,8 @@ cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream) {
   a.per = p.Hk * a.n_group / a.heads;
   a.runs = p.num_sms;
   const long long rows = (long long)p.B * p.Hk * a.R;
-  const long long units = head_steps_of(p) * ((p.max_len + UNIT - 1) / UNIT);
-  if (rows > 0x3fffffffLL || units > 0x3fffffffLL) return cudaErrorInvalidValue;  // both are numbered in 32 bits
+  const long long places = head_steps_of(p) * ((p.max_len + UNIT - 1) / UNIT + ENTRY);
+  if (rows > 0x3fffffffLL || places > 0x3fffffffLL) return cudaErrorInvalidValue;  // both are numbered in 32 bits
   if (p.scratch == nullptr) return cudaErrorInvalidValue;
   a.part_o = p.scratch;
   a.part_ml = reinterpret_cast<float2*>(p.scratch + (size_t)partials_of(p) * HD);
