@@ -42,7 +42,8 @@ constexpr int MAX_T = kMoeDecMaxTokens;
 constexpr int MAX_E = kMoeDecMaxExperts;
 constexpr int MAX_K = kMoeDecMaxTopk;
 constexpr int MAX_SLOTS = MAX_T * MAX_K;
-constexpr int NTHREADS = 192;           // warp 0 TMA, 1 MMA, 2-5 epilogue
+constexpr int EPI_WARPS = 4;
+constexpr int NTHREADS = 256;           // warp 0 TMA, 1 MMA, 2-5 epilogue; all of them build the tables
 constexpr int MAX_STAGES = 12;
 constexpr int MIN_CHUNKS = 4;           // a CTA takes at least this many weight tiles
 constexpr int TMEM_COLS = 2 * MAX_T;    // two accumulators
@@ -137,9 +138,9 @@ __global__ void __launch_bounds__(32 * LOGIT_WARPS) moe_logits_kernel(const __gr
 }
 
 // A token's experts by repeated maximum, by a whole warp: equal logits go to the lower expert, NaN
-// counts as the largest. Lane k < topk gets choice k and its weight.
+// counts as the largest. Lane k < topk gets choice k and its logit.
 template <int PER>  // experts a lane
-__device__ __forceinline__ void choose(const Args& a, int t, int lane, int& mine_e, float& mine_w) {
+__device__ __forceinline__ void choose(const Args& a, int t, int lane, int& mine_e, float& mine) {
   float v[PER];
   uint32_t key[PER];
 #pragma unroll
@@ -149,32 +150,29 @@ __device__ __forceinline__ void choose(const Args& a, int t, int lane, int& mine
     key[i] = v[i] != v[i] ? 0xffffffffu : (v[i] == 0.f ? 0x80000000u : (b & 0x80000000u ? ~b : b | 0x80000000u));
     if (i * 32 + lane >= a.E) key[i] = 0;  // below every number: -infinity is 0x007fffff
   }
-  float top = 0.f, sum = 0.f, mine = 0.f;
   mine_e = 0;
+  mine = 0.f;
   for (int k = 0; k < a.topk; k++) {
-    uint32_t best = 0;
+    uint32_t best = key[0];
 #pragma unroll
-    for (int i = 0; i < PER; i++) best = max(best, key[i]);
+    for (int i = 1; i < PER; i++) best = max(best, key[i]);
     best = __reduce_max_sync(0xffffffffu, best);
-    unsigned int e = MAX_E;
+    unsigned int chosen = 0;
     float val = 0.f;
 #pragma unroll
-    for (int i = PER - 1; i >= 0; i--)
-      if (key[i] == best) e = i * 32 + lane, val = v[i];
-    const unsigned int chosen = __reduce_min_sync(0xffffffffu, e);
+    for (int i = PER - 1; i >= 0; i--) {  // the lowest group that holds it, and its lowest lane
+      const unsigned int m = __ballot_sync(0xffffffffu, key[i] == best);
+      if (m) chosen = i * 32 + __ffs(m) - 1, val = v[i];
+    }
     val = __shfl_sync(0xffffffffu, val, chosen & 31);
 #pragma unroll
     for (int i = 0; i < PER; i++)
       if (i * 32 + lane == chosen) key[i] = 0;
-    if (k == 0) top = val;
-    const float p = expf(val - top);
-    sum += p;
     if (lane == k) {
-      mine = p;
+      mine = val;
       mine_e = (int)chosen;
     }
   }
-  mine_w = mine / sum;
 }
 
 // ------------------------------------------------------------------------------------ the products
@@ -214,12 +212,17 @@ __device__ void build_tables(Tables& tb, const Args& a, bool keep_weights) {
   if (threadIdx.x == 0) tb.most = 0;
   for (int t = warp; t < a.T; t += NTHREADS / 32) {
     int e;
-    float w;
-    if (a.E <= 32) choose<1>(a, t, lane, e, w);
-    else choose<MAX_E / 32>(a, t, lane, e, w);
-    if (lane < a.topk) {
-      tb.id[t * a.topk + lane] = (short)e;
-      if (keep_weights) a.wts[t * a.topk + lane] = w;
+    float v;
+    if (a.E <= 32) choose<1>(a, t, lane, e, v);
+    else choose<MAX_E / 32>(a, t, lane, e, v);
+    if (lane < a.topk) tb.id[t * a.topk + lane] = (short)e;
+    if (keep_weights) {  // softmax over the choices; the first is the largest
+      const float top = __shfl_sync(0xffffffffu, v, 0);  // by every lane: a shuffle in a branch would wait for the others
+      const float p = lane < a.topk ? expf(v - top) : 0.f;
+      float sum = p;
+#pragma unroll
+      for (int o = MAX_K / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane < a.topk) a.wts[t * a.topk + lane] = p / sum;
     }
   }
   if (threadIdx.x < 16 && a.slots + threadIdx.x < MAX_SLOTS) tb.id[a.slots + threadIdx.x] = MAX_E;  // no expert
@@ -303,7 +306,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&sm.tfull[b], 1);
-      mbar_init(&sm.tempty[b], 4);
+      mbar_init(&sm.tempty[b], EPI_WARPS);
     }
     mbar_init(&sm.drain, 1);
     fence_barrier_init();
@@ -470,7 +473,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
         }
       }
     }
-  } else {
+  } else if (warp < 2 + EPI_WARPS) {
     if (!UP) {
       pdl_wait();  // the partial sums' memory may be in use until here
       pdl_launch();
@@ -536,13 +539,13 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           float* const mine = tile(cta);
           columns([&](int j, float v) { __stcg(mine + (long long)j * BM, v); });
           release();
-          asm volatile("bar.sync 1, 128;" ::: "memory");  // with the fence: every thread's part is there before the count
+          asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");  // with the fence: every thread's part is there before the count
           if (threadIdx.x == 64) {
             __threadfence();
             sm.last = atomicAdd(a.done + item, 1u) == (unsigned)(c1 - c0);
             __threadfence();
           }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+          asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");
           if (sm.last) {
             constexpr int COLS = 4;  // columns in flight
             for (int j0 = 0; j0 < n; j0 += COLS) {
@@ -580,28 +583,35 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
 __global__ void __launch_bounds__(128) moe_combine_kernel(const __grid_constant__ Args a, int grid) {
   const int t = blockIdx.y, d = (blockIdx.x * 128 + threadIdx.x) * 2;
-  pdl_wait();
-  pdl_launch();
-  if (d >= a.D) return;
-  // every load of the choices before the first use, then the first two partial sums of each
+  // The choices and the residual are there: this kernel starts only after every CTA of the down product
+  // has waited for the gate/up product. Only the partial sums are read after its own wait, the first
+  // two of every choice before their first use.
+  const bool mine = d < a.D;
   int at[MAX_K], n[MAX_K];
   float w[MAX_K];
-  float2 v[MAX_K], u[MAX_K];
 #pragma unroll
   for (int k = 0; k < MAX_K; k++) {
     const int i = t * a.topk + min(k, a.topk - 1);
     at[k] = __ldcg(a.place + i);
     w[k] = __ldcg(a.wts + i);
   }
+  const uint32_t r = a.residual && mine ? *reinterpret_cast<const uint32_t*>(a.residual + t * a.ldres + d) : 0u;
   const Stream st(__ldcg(a.place + a.slots), (a.D + BM - 1) / BM, (a.F + BK - 1) / BK, grid);
+#pragma unroll
+  for (int k = 0; k < MAX_K; k++) {
+    const int item = (at[k] >> 16) * st.rt + min(d, a.D - 1) / BM;
+    n[k] = st.owner((item + 1) * st.kc - 1) - st.owner(item * st.kc) + 1;
+    at[k] &= 0xffff;
+  }
+  pdl_wait();
+  pdl_launch();
+  if (!mine) return;
   const float* const y = a.y + d;
   const long long part = (long long)a.slots * a.D;
+  float2 v[MAX_K], u[MAX_K];
 #pragma unroll
   for (int k = 0; k < MAX_K; k++) {
     if (k >= a.topk) break;
-    const int item = (at[k] >> 16) * st.rt + d / BM;
-    n[k] = st.owner((item + 1) * st.kc - 1) - st.owner(item * st.kc) + 1;
-    at[k] &= 0xffff;
     v[k] = __ldcg(reinterpret_cast<const float2*>(y + (long long)at[k] * a.D));
     u[k] = make_float2(0.f, 0.f);
     if (n[k] > 1) u[k] = __ldcg(reinterpret_cast<const float2*>(y + part + (long long)at[k] * a.D));
@@ -619,11 +629,8 @@ __global__ void __launch_bounds__(128) moe_combine_kernel(const __grid_constant_
     s0 = fmaf(w[k], y0, s0);
     s1 = fmaf(w[k], y1, s1);
   }
-  if (a.residual) {
-    const uint32_t r = *reinterpret_cast<const uint32_t*>(a.residual + t * a.ldres + d);
-    s0 += __uint_as_float(r << 16);
-    s1 += __uint_as_float(r & 0xffff0000u);
-  }
+  s0 += __uint_as_float(r << 16);
+  s1 += __uint_as_float(r & 0xffff0000u);
   *reinterpret_cast<uint32_t*>(a.out + t * a.ldo + d) = pack_bf16x2(s0, s1);
 }
 
