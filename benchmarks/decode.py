@@ -7,6 +7,9 @@ Shapes (B sequences, context, query heads, KV heads):
   llama70b_tp8  32 x 2304,  8 / 1   (one rank's heads at TP = 8)
   mixtral       64 x 1152, 48 / 8   (1024 prompt + 128 decode tokens)
 
+``--caches int8,e4m3`` also times ``ops.decode_attention_q8`` over the same keys and values in 8 bits
+(written by ``ops.kv_append_q8``, whose time for the whole context is given too).
+
 For each: the split-KV decode kernel (``ops.decode_attention``), the prefill kernel given one
 query per sequence (``ops.attention``, what the decode path used before), and PyTorch SDPA
 (``enable_gqa``). Times are CUDA-event medians of device time (the GPU is given a head start so
@@ -62,6 +65,7 @@ def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--shapes", default="llama70b,llama70b_tp8,mixtral")
     ap.add_argument("--iters", type=int, default=20)
+    ap.add_argument("--caches", default="int8,e4m3", help="8-bit formats to time as well (empty: none)")
     ap.add_argument("--n-split", type=int, default=0, help="0: the library's choice")
     a = ap.parse_args()
     from flextensor_b200 import ops
@@ -91,6 +95,21 @@ def main():
                           "n_split": a.n_split or native.lib().decode_splits(B, Hk, L, torch.cuda.get_device_properties(dev).multi_processor_count),
                           "decode_x_roofline": round(t_dec / roof_us, 2), "prefill_kernel_us": round(t_pre, 1),
                           "sdpa_us": round(t_sdpa, 1), "max_abs_diff_vs_prefill_kernel": err}))
+        for fmt in [f for f in a.caches.split(",") if f]:
+            dt = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}[fmt]
+            cache = [torch.zeros(B, L, Hk, 128, device=dev, dtype=dt) for _ in range(2)]
+            cache += [torch.zeros(B, -(-L // 64), Hk, device=dev) for _ in range(2)]
+            t_app = timed(lambda: ops.kv_append_q8(kc, vc, *cache, 0), a.iters, flush)
+            t_tok = timed(lambda: ops.kv_append_q8(kc[:, -1:], vc[:, -1:], *cache, L - 1), a.iters, flush)
+            t_q8 = timed(lambda: ops.decode_attention_q8(q, *cache, L, out=out), a.iters, flush)
+            q8_bytes = 2 * B * L * Hk * 128 + 2 * 4 * cache[2].numel()
+            diff = ((out.float() - ops.decode_attention(q, kc, vc, L).float()).norm() / out.float().norm()).item()
+            assert native.device_error(reset=True) == 0
+            print(json.dumps({"shape": name, "cache": fmt, "kv_MB": round(q8_bytes / 1e6, 1),
+                              "roofline_us": round(q8_bytes / (bw * 1e3), 1), "decode_q8_us": round(t_q8, 1),
+                              "x_bf16_kernel": round(t_dec / t_q8, 2), "append_context_us": round(t_app, 1),
+                              "append_token_us": round(t_tok, 1), "rel_diff_vs_bf16_cache": round(diff, 5)}))
+            del cache
 
 
 if __name__ == "__main__":

@@ -153,7 +153,7 @@ def kv_append_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     ``[B]``. ``n_new`` (int32 CUDA ``[B]``): tokens to take of each sequence's S; the rest are
     padding, not read.
 
-    A block's scale is the smallest power of two with ``max|x| <= 127 * scale`` (448 for e4m3; 0
+    Codes and scales start as zeros. A block's scale is the smallest power of two with ``max|x| <= 127 * scale`` (448 for e4m3; 0
     for a block of zeros, never below 2**-120). A block whose first position is written starts
     afresh; one that holds earlier tokens of the sequence keeps the larger of its scale and the new
     tokens', and its codes are rounded again when that grows. A NaN or infinity makes its block's
@@ -175,7 +175,7 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     scales that are not negative; e4m3 codes must be finite).
 
     ``q [B, Hq, 128]``, or ``[B, Sq, Hq, 128]`` for the last Sq tokens of each sequence, whose keys
-    are in the cache already: query i sees keys ``[0, kv_len - Sq + 1 + i)``; one that sees none
+    are in the cache already (a few: the workspace grows with Sq): query i sees keys ``[0, kv_len - Sq + 1 + i)``; one that sees none
     gets zeros. ``kv_len``: an int or an int32 CUDA tensor ``[B]`` (then ``max_len``, default L,
     bounds it: longer ones are cut)."""
     if scale is None:

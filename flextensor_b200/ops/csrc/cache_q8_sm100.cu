@@ -44,6 +44,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "ft_cache.h"
 #include "ft_ops.h"
@@ -937,12 +938,14 @@ bool side_map(CUtensorMap* m, const CacheSide& s, const CacheDecodeProblem& p, i
 template <int NT, int FMT>
 cudaError_t launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const DecArgs& a, int sms, cudaStream_t stream) {
   const int smem = (int)sizeof(DecSmem<NT>) + 1024;
-  static bool attr = false;
-  if (!attr) {
-    const cudaError_t e = cudaFuncSetAttribute(cache_decode_kernel<NT, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    attr = true;
+  static std::atomic<bool> ready[64];  // the attribute belongs to a kernel on one device
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess && (dev >= 64 || !ready[dev])) {
+    err = cudaFuncSetAttribute(cache_decode_kernel<NT, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err == cudaSuccess && dev < 64) ready[dev] = true;
   }
+  if (err != cudaSuccess) return err;
   const cudaError_t e =
       launch_overlapped(cache_decode_kernel<NT, FMT>, (unsigned)sms, 32 * WARPS, smem, stream, tk, tv, a);
   if (e != cudaSuccess) return e;

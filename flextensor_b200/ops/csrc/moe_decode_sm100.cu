@@ -24,6 +24,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "ft_moe_decode.h"
 #include "ft_ops.h"
@@ -726,13 +727,14 @@ cudaError_t launch_product(const MoeDecodeProblem& p, Args a, cudaStream_t strea
   }
   if (!ok) return cudaErrorInvalidValue;
   const int smem = RING_BUDGET + 1024;
-  static bool attr = false;
-  if (!attr) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(moe_product_kernel<UP, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    attr = true;
+  static std::atomic<bool> ready[64];  // the attribute belongs to a kernel on one device
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess && (dev >= 64 || !ready[dev])) {
+    err = cudaFuncSetAttribute(moe_product_kernel<UP, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (err == cudaSuccess && dev < 64) ready[dev] = true;
   }
+  if (err != cudaSuccess) return err;
   return launch_overlapped(moe_product_kernel<UP, N>, dim3((unsigned)p.num_sms), NTHREADS, smem, stream, tm_b, tm_lo, maps, a);
 }
 

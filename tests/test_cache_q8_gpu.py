@@ -232,6 +232,20 @@ def test_attention_bounds_and_strides():
     check_attend(q, view, [L] * B, block, L)
 
 
+def test_attention_over_a_shared_cache():
+    """A cache expanded over sequences (one prompt for several), or over heads; q expanded too; out = q."""
+    B, L, Hq, Hk, block = 5, 230, 16, 2, 64
+    lens = torch.tensor([230, 1, 64, 100, 0], dtype=torch.int32, device=DEV)
+    one = junk_cache("e4m3", 1, L, Hk, block, 21)
+    q = bf16(22, B, Hq, 128, spread=False)
+    check_attend(q, [c.expand(B, *c.shape[1:]) for c in one], lens, block, lens)
+    narrow = junk_cache("int8", B, L, 1, block, 23)
+    wide = [narrow[0].expand(B, L, Hk, 128), narrow[1].expand(B, L, Hk, 128), narrow[2].expand(B, -1, Hk), narrow[3].expand(B, -1, Hk)]
+    want = check_attend(q[:1].expand(B, Hq, 128), wide, lens, block, lens)
+    mine = q[:1].expand(B, Hq, 128).contiguous()
+    assert torch.equal(ops.decode_attention_q8(mine, *wide, lens, block=block, out=mine), want)
+
+
 def test_attention_scales_and_magnitudes():
     """Value scales 2^40 apart between blocks, zero scales, queries near the type's limits."""
     B, L, Hq, Hk, block = 1, 128, 8, 1, 16

@@ -1,0 +1,111 @@
+"""CPU model of how ``ops/csrc/cache_q8_sm100.cu`` divides attention over an 8-bit cache: the sequence of
+places (``ENTRY`` per head and sequence, then its 32-key units) is cut into equal runs, one per CTA; a
+CTA's warps take tiles of their heads from it and write partial results; the merge finds them again by
+arithmetic alone. Checked for random ragged batches: every unit of every head is taken exactly once, a
+warp's partials have distinct numbers within the workspace, and the merge counts exactly those written."""
+
+import random
+
+import pytest
+
+WARPS, ENTRY = 8, 1
+
+
+class Runs:
+    def __init__(self, total, most):
+        self.n = min(most, total)
+        self.base = total // self.n if self.n else 0
+        self.rem = total - self.base * self.n
+
+    def begin(self, r):
+        return r * self.base + min(r, self.rem)
+
+    def owner(self, i):
+        longer = self.rem * (self.base + 1)
+        return i // (self.base + 1) if i < longer else self.rem + (i - longer) // self.base
+
+
+def side_by_side(u):
+    return next(h for h in (8, 4, 2, 1) if u % h == 0)
+
+
+def taken(lens, heads_groups, ut, sms):
+    """{(b, head group): {unit: times}}, {(b, head group): [(run, key warp)]}, the highest partial number."""
+    units = [-(-n // 32) for n in lens]
+    cost = [n + ENTRY if n else 0 for n in units]
+    heads = side_by_side(heads_groups)
+    keys, per = WARPS // heads, heads_groups // heads
+    runs = Runs(sum(cost) * per, sms)
+    got, partials, seen = {}, {}, set()
+    for run in range(runs.n):
+        first, count = runs.begin(run), runs.begin(run + 1) - runs.begin(run)
+        for warp in range(WARPS):
+            my_head, start, step = warp % heads, warp // heads * ut, keys * ut
+            # locate
+            i, b = first, 0
+            while i >= cost[b] * per:
+                i -= cost[b] * per
+                b += 1
+            n = cost[b]
+            j, i = divmod(i, n)
+            left = count - (min(n, i + count) - i)
+            t, end = max(0, i - ENTRY) + start, min(n, i + count) - ENTRY
+            while True:
+                done = False
+                while t >= end:
+                    if left == 0:
+                        done = True
+                        break
+                    j += 1
+                    if j == per:
+                        j, b = 0, b + 1
+                    while cost[b] == 0:
+                        b += 1
+                    n = min(cost[b], left)
+                    left -= n
+                    end, t = n - ENTRY, start
+                if done:
+                    break
+                hg = j * heads + my_head
+                for u in range(t, min(t + ut, end)):
+                    d = got.setdefault((b, hg), {})
+                    d[u] = d.get(u, 0) + 1
+                key = (run, warp // heads)
+                if key not in partials.setdefault((b, hg), []):
+                    partials[b, hg].append(key)
+                    number = (b * per + j + run) * WARPS + warp
+                    assert number not in seen
+                    seen.add(number)
+                t += step
+    assert not seen or max(seen) < (len(lens) * per + sms) * WARPS
+    return got, partials
+
+
+def merged(lens, heads_groups, ut, sms, b, hg):
+    units = [-(-n // 32) for n in lens]
+    cost = [n + ENTRY if n else 0 for n in units]
+    heads = side_by_side(heads_groups)
+    keys, per = WARPS // heads, heads_groups // heads
+    runs = Runs(sum(cost) * per, sms)
+    f, n = sum(cost[:b]) * per + hg // heads * cost[b], cost[b]
+    r0, out = runs.owner(f), []
+    for i in range((runs.owner(f + n - 1) + 1 - r0) * keys):
+        run = r0 + i // keys
+        lo, hi = max(f, runs.begin(run)) - f, min(f + n, runs.begin(run + 1)) - f
+        if max(0, lo - ENTRY) + i % keys * ut < hi - ENTRY:
+            out.append((run, i % keys))
+    return out
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_runs(seed):
+    rng = random.Random(seed)
+    B, hgs, ut, sms = rng.randint(1, 9), rng.choice([1, 2, 3, 4, 5, 8, 12, 16]), rng.choice([1, 2]), rng.choice([3, 13, 148])
+    lens = [rng.choice([0, 1, 31, 32, 33, 64, rng.randint(1, 700), rng.randint(1, 3000)]) for _ in range(B)]
+    got, partials = taken(lens, hgs, ut, sms)
+    for b, n in enumerate(lens):
+        for hg in range(hgs):
+            units = -(-n // 32)
+            assert got.get((b, hg), {}) == {u: 1 for u in range(units)}
+            if units:
+                assert merged(lens, hgs, ut, sms, b, hg) == sorted(partials[b, hg])

@@ -75,8 +75,10 @@ def test_stream_partition_model():
         rt, kc = -(-D_ // 128), -(-F_ // 64)
         total = n_act * rt * kc
         ctas = min(sms, max(1, total // 4))
-        begin = lambda c: total * c // ctas  # noqa: E731
-        owner = lambda i: ((i + 1) * ctas - 1) // total  # noqa: E731
+        base, rem = divmod(total, ctas)
+        begin = lambda c: c * base + min(c, rem)  # noqa: E731
+        longer = rem * (base + 1)
+        owner = lambda i: i // (base + 1) if i < longer else rem + (i - longer) // base  # noqa: E731
         assert begin(0) == 0 and begin(ctas) == total
         for c in range(ctas):
             assert begin(c) < begin(c + 1) and owner(begin(c)) == c == owner(begin(c + 1) - 1)

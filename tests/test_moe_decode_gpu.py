@@ -87,6 +87,14 @@ def test_strides_and_aliases():
     assert torch.equal(ops.moe_decode(**p, topk=2, residual=one), ops.moe_decode(**p, topk=2))
 
 
+def test_shared_and_scattered_experts():
+    """The same weights for every expert, and experts in no order of memory."""
+    p, res = make(5, 256, 192, 4, seed=7)
+    check(dict(p, w_gate_up=[p["w_gate_up"][0]] * 4, w_down=[p["w_down"][3]] * 4), 2, residual=res)
+    order = [2, 0, 3, 1]
+    check(dict(p, w_gate_up=[p["w_gate_up"][i] for i in order], w_down=[p["w_down"][i] for i in order]), 3)
+
+
 def test_routing_corners():
     """All tokens on one expert; equal logits go to the lowest expert; a NaN token stays alone; weights
     that are NaN for an expert that nobody chose are not touched."""
