@@ -34,8 +34,9 @@
 // overlaps the first one's end, merges the partials of each row in a fixed order.
 //
 // Scales: a score is (q . codes) * ks, and the weight of a value's codes is p * vs. The running
-// reference m is the maximum of score + log2(vs), so p * vs <= 1 whatever the scales are and f16
-// holds it to 2^-11 of the largest weight; the sum l takes p itself in fp32. q is scaled by a power
+// reference is 7 below the maximum of score + log2(vs) (in log2 units), so that p * vs is at most 2^15
+// whatever the scales are and f16 holds it to 2^-11, or to 2^-32 of the largest weight where that is
+// more (a million keys that weigh less together still add up to 2^-12); the sum l takes p in fp32. q is scaled by a power
 // of two per row into f16 (exact but for elements below 2^-24 of the row's largest).
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -128,7 +129,9 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
 }
 
 // One CTA per (sequence, block of tokens, KV head, keys or values); the block's new tokens are
-// held in registers between the maximum and the rounding, so they are read once.
+// held in registers between the maximum and the rounding, so they are read once. Bound by HBM for
+// prompts (32 x 2048 tokens, 8 heads: 403 MB in 73 us, 5.5 TB/s) and by the launch for single
+// tokens (32 sequences: 3.0 us on the device).
 template <int BLOCK, int FMT>
 __global__ void __launch_bounds__(BLOCK <= 64 ? 128 : 256) cache_append_kernel(AppendArgs a) {
   constexpr int THREADS = BLOCK <= 64 ? 128 : 256;
@@ -454,16 +457,16 @@ __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT
 #pragma unroll
       for (int mt = 1; mt < MT; mt++) top[i] = max_nan(top[i], max_nan(s[mt][nt][i], s[mt][nt][2 + i]) + lv[mt]);
     }
-    // the reference moves only when a weight would pass 2^8 (f16 holds 2^15), so the accumulators are
-    // seldom rescaled; all lanes of a column take the same one
-    const bool grow = !(top[0] <= st.m[nt][0] + 8.f) || !(top[1] <= st.m[nt][1] + 8.f);
+    // the reference moves only when a weight would pass 2^15, so the accumulators are seldom rescaled;
+    // all lanes of a column take the same one
+    const bool grow = !(top[0] <= st.m[nt][0] + 15.f) || !(top[1] <= st.m[nt][1] + 15.f);
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 4));
         top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 8));
         top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
-        const float m_new = max_nan(st.m[nt][i], top[i]);
+        const float m_new = max_nan(st.m[nt][i], top[i] - 7.f);
         const float al = st.m[nt][i] == -INFINITY ? 0.f : ex2f(st.m[nt][i] - m_new);
         st.m[nt][i] = m_new;
         st.l[nt][i] *= al;
@@ -640,6 +643,10 @@ struct DecSmem {
   uint64_t full[WARPS][SLOTS];
 };
 
+// Bound by HBM where sequences are long (131071 tokens, 8 heads, e4m3: 268 MB in 49 us with the merge,
+// 5.4 TB/s; 32 x 2304 tokens, int8: 151 MB in 36 us, of which 24 us stream) and by latency where they
+// are short. The loads of a head's queries and scales come before the copies, which would hold them
+// up for 5 us in the memory's queues.
 template <int NT, int FMT>
 __global__ void __launch_bounds__(32 * WARPS, 1)
     cache_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -812,7 +819,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
 }
 
 // Rows of the output: each row's partial results in the order of runs and warps, `merge_per_row` warps a
-// row (each a contiguous part of them), four dims a lane, eight partials in flight.
+// row (each a contiguous part of them), four dims a lane, eight partials in flight. Bound by latency:
+// 1.6 us after its wait for 2048 rows of some six partials each.
 template <int NT>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(const __grid_constant__ DecArgs a) {
   __shared__ float4 so[MERGE_WARPS][32];

@@ -264,6 +264,26 @@ def test_attention_scales_and_magnitudes():
     check_attend((q.float() * 2.0 ** -108).bfloat16(), cache, [L], block, L)
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_attention_many_small_weights(fmt):
+    """One key outweighs each of 131071 others by e^18 = 2^26, and its value is zero: the output is what
+    the others add up to, although each of their weights is below f16's steps next to 1."""
+    L, block = 131072, 256
+    cache = new_cache(fmt, 1, L, 1, block)
+    one = 64 if fmt == "int8" else 64.0
+    cache[0][..., 0] = one                        # every key: 64 in dim 0 ...
+    cache[0][0, 70001, 0, 1] = one                # ... the heavy one 64 in dim 1 too
+    cache[1].copy_(torch.full((), one, device=DEV).expand(1, L, 1, 128).to(FMT[fmt]))
+    cache[1][0, 70001] = 0
+    cache[2].fill_(2.0 ** -6)
+    cache[3].fill_(2.0 ** -6)
+    q = torch.zeros(1, 8, 128, device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    q[..., 1] = 18.0 * 128 ** 0.5
+    got = check_attend(q, cache, [L], block, L)
+    assert 1e-3 < float(got.min()) and float(got.max()) < 3e-3
+
+
 def test_attention_keeps_nan():
     """A NaN block reaches exactly the rows that see it, through keys or values alike."""
     B, Sq, L, Hq, Hk, block = 2, 3, 96, 4, 1, 32
