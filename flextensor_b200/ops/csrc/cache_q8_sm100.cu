@@ -82,7 +82,7 @@ cudaError_t launch_overlapped(void (*kernel)(P...), unsigned grid, int threads, 
 
 // ------------------------------------------------------------------------------------ writing
 struct AppendArgs {
-  int B, S, Hk, L, n_rel;
+  int B, S, Hk, L, n_rel;  // n_rel: groups of blocks a sequence can touch, one a CTA
   const __nv_bfloat16* x[2];
   long long x_b[2], x_tok[2], x_h[2];
   CacheSide side[2];
@@ -102,11 +102,14 @@ __device__ __forceinline__ float pow2_scale(uint32_t bits) {
   return __int_as_float((max(k, -120) + 127) << 23);
 }
 
+// Four values to codes, rounded to nearest even. int8: the sum with 1.5 * 2^23 has the rounded number in
+// its low bits; values are within +-128 by the choice of the scale. (The integer conversion runs at a
+// quarter of the rate: prompts took 72 us with it, 61 without.)
 template <int FMT>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
   if (FMT == CACHE_INT8) {
-    const int ia = min(127, max(-127, __float2int_rn(a))), ib = min(127, max(-127, __float2int_rn(b)));
-    const int ic = min(127, max(-127, __float2int_rn(c))), id = min(127, max(-127, __float2int_rn(d)));
+    const uint32_t ia = __float_as_uint(a + 12582912.f), ib = __float_as_uint(b + 12582912.f);
+    const uint32_t ic = __float_as_uint(c + 12582912.f), id = __float_as_uint(d + 12582912.f);
     return __byte_perm(__byte_perm(ia, ib, 0x0040), __byte_perm(ic, id, 0x0040), 0x5410);
   }
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
@@ -128,22 +131,30 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
   return encode4<FMT>(f[0] * ratio, f[1] * ratio, f[2] * ratio, f[3] * ratio);
 }
 
-// One CTA per (sequence, block of tokens, KV head, keys or values); the block's new tokens are
-// held in registers between the maximum and the rounding, so they are read once. Bound by HBM for
-// prompts (32 x 2048 tokens, 8 heads: 403 MB in 73 us, 5.5 TB/s) and by the launch for single
-// tokens (32 sequences: 3.0 us on the device).
+// A block belongs to BLOCK / 16 warps, whose lanes hold its new tokens in registers (eight 16-byte pieces
+// each) between the maximum and the rounding, so they are read once; a CTA of at least four warps takes
+// consecutive blocks of one sequence and KV head, keys or values. Bound by HBM for prompts (32 x 2048
+// tokens, 8 heads: 403 MB in 61-63 us at blocks of 16 to 64 tokens, the rate of a copy; 66 at 128, 94 at
+// 256, where few large CTAs overlap their loads and stores badly) and by the launch for single tokens
+// (3.0 us on the device).
+template <int BLOCK>
+struct AppendShape {
+  static constexpr int WARPS_PER_BLOCK = BLOCK / 16, WARPS = WARPS_PER_BLOCK > 4 ? WARPS_PER_BLOCK : 4;
+  static constexpr int BLOCKS = WARPS / WARPS_PER_BLOCK;  // of a CTA
+};
+
 template <int BLOCK, int FMT>
-__global__ void __launch_bounds__(BLOCK <= 64 ? 128 : 256) cache_append_kernel(AppendArgs a) {
-  constexpr int THREADS = BLOCK <= 64 ? 128 : 256;
-  constexpr int ROWS = THREADS / 16;  // token rows per pass: 16 lanes hold a row's 128 values
-  constexpr int ITERS = BLOCK / ROWS;
-  __shared__ uint32_t warp_max[THREADS / 32];
+__global__ void __launch_bounds__(32 * AppendShape<BLOCK>::WARPS) cache_append_kernel(const __grid_constant__ AppendArgs a) {
+  using Shape = AppendShape<BLOCK>;
+  constexpr int WPB = Shape::WARPS_PER_BLOCK, STEP = 2 * WPB, ITERS = 8;  // a warp's pass is two token rows
+  __shared__ uint32_t warp_max[Shape::WARPS];
   pdl_wait();
   pdl_launch();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   long long id = blockIdx.x;
   const int h = (int)(id % a.Hk);
   id /= a.Hk;
-  const int rel = (int)(id % a.n_rel);
+  const int rel = (int)(id % a.n_rel) * Shape::BLOCKS + warp / WPB;
   id /= a.n_rel;
   const int kv = (int)(id & 1), b = (int)(id >> 1);
   const int p = a.pos ? a.pos[b] : a.pos_all, n = a.n_new ? a.n_new[b] : a.S;
@@ -152,19 +163,18 @@ __global__ void __launch_bounds__(BLOCK <= 64 ? 128 : 256) cache_append_kernel(A
     return;
   }
   const int j = p / BLOCK + rel;
-  const int t0 = max(p, j * BLOCK), t1 = min(p + n, (j + 1) * BLOCK);
-  if (t0 >= t1) return;
+  const int t0 = max(p, j * BLOCK), t1 = min(p + n, (j + 1) * BLOCK);  // new tokens of the block; t0 >= t1: none
   const CacheSide& sd = a.side[kv];
   float* const sp = sd.scale + b * sd.s_b + j * sd.s_blk + h * sd.s_h;
-  const bool history = t0 > j * BLOCK;
+  const bool some = t0 < t1, history = some && t0 > j * BLOCK;
   const float s_old = history ? *sp : 0.f;
-  const int row0 = threadIdx.x / 16, col = (threadIdx.x % 16) * 8;
+  const int row0 = j * BLOCK + (warp % WPB) * 2 + lane / 16, col = (lane % 16) * 8;
   const __nv_bfloat16* const x = a.x[kv] + b * a.x_b[kv] + h * a.x_h[kv] + col;
   uint4 v[ITERS];
   uint32_t m2 = 0;
 #pragma unroll
   for (int i = 0; i < ITERS; i++) {
-    const int t = j * BLOCK + i * ROWS + row0;
+    const int t = row0 + i * STEP;
     v[i] = make_uint4(0, 0, 0, 0);
     if (t >= t0 && t < t1) v[i] = *reinterpret_cast<const uint4*>(x + (long long)(t - p) * a.x_tok[kv]);
   }
@@ -174,10 +184,15 @@ __global__ void __launch_bounds__(BLOCK <= 64 ? 128 : 256) cache_append_kernel(A
                                __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
   }
   uint32_t m = __reduce_max_sync(0xffffffffu, max(m2 & 0xffffu, m2 >> 16));
-  if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
-  __syncthreads();  // also: every thread has read the old scale
+  if (WPB > 1) {
+    if (lane == 0) warp_max[warp] = m;
+    __syncthreads();  // also: every thread has read the old scale
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; w++) m = max(m, warp_max[w]);
+    for (int w = 0; w < WPB; w++) m = max(m, warp_max[warp / WPB * WPB + w]);
+  } else {
+    __syncwarp();
+  }
+  if (!some) return;
   const float s_new = pow2_scale<FMT>(m);
   const float s = s_old != s_old ? s_old : (s_new != s_new ? s_new : fmaxf(s_old, s_new));
   const bool bad = s != s;
@@ -185,16 +200,16 @@ __global__ void __launch_bounds__(BLOCK <= 64 ? 128 : 256) cache_append_kernel(A
   uint8_t* const out = sd.codes + b * sd.c_b + h * sd.c_h + col;
   if (history && s != s_old) {
     const float ratio = bad ? 0.f : s_old * inv;
-    for (int t = j * BLOCK + row0; t < t0; t += ROWS) {
+    for (int t = row0; t < t0; t += STEP) {
       uint2* const w = reinterpret_cast<uint2*>(out + (long long)t * sd.c_tok);
       const uint2 o = *w;
       *w = bad ? make_uint2(0, 0) : make_uint2(recode4<FMT>(o.x, ratio), recode4<FMT>(o.y, ratio));
     }
   }
-  if (threadIdx.x == 0) *sp = s;
+  if (lane == 0 && warp % WPB == 0) *sp = s;
 #pragma unroll
   for (int i = 0; i < ITERS; i++) {
-    const int t = j * BLOCK + i * ROWS + row0;
+    const int t = row0 + i * STEP;
     if (t < t0 || t >= t1) continue;
     const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
     float f[8];
@@ -210,12 +225,13 @@ __global__ void __launch_bounds__(BLOCK <= 64 ? 128 : 256) cache_append_kernel(A
 }
 
 template <int BLOCK>
-cudaError_t launch_append(const AppendArgs& a, int format, cudaStream_t stream) {
+cudaError_t launch_append(AppendArgs a, int format, cudaStream_t stream) {
+  using Shape = AppendShape<BLOCK>;
+  a.n_rel = (a.n_rel + Shape::BLOCKS - 1) / Shape::BLOCKS;
   const long long grid = (long long)a.B * 2 * a.n_rel * a.Hk;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const int threads = BLOCK <= 64 ? 128 : 256;
   return launch_overlapped(format == CACHE_INT8 ? cache_append_kernel<BLOCK, CACHE_INT8> : cache_append_kernel<BLOCK, CACHE_E4M3>,
-                           (unsigned)grid, threads, 0, stream, a);
+                           (unsigned)grid, 32 * Shape::WARPS, 0, stream, a);
 }
 
 // ------------------------------------------------------------------------------------ attention
