@@ -243,7 +243,7 @@ constexpr int units_of_tile(int column_tiles) { return column_tiles == 1 ? 2 : 1
 constexpr int UNIT_BYTES = UNIT * HD;
 // What entering a head costs a warp (its queries, its partial result, a tile cut short), in units: runs
 // are equal in units plus this much for each head and sequence
-constexpr int ENTRY = 1;
+constexpr int ENTRY = 2;
 constexpr int MERGE_WARPS = 16;  // at most
 
 struct DecArgs {

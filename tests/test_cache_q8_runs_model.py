@@ -8,7 +8,7 @@ import random
 
 import pytest
 
-WARPS, ENTRY = 8, 1
+WARPS, ENTRY = 8, 2
 
 
 class Runs:
