@@ -164,7 +164,7 @@ def kv_append_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
         native.lib().kv_append_q8(k, v, k_cache, v_cache, k_scale, v_scale, pos, 0, n_new, block)
     else:
         native.lib().kv_append_q8(k, v, k_cache, v_cache, k_scale, v_scale, None, pos, n_new, block)
-    _count()
+    _count(1 if k.shape[1] else 0)
 
 
 def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -186,7 +186,7 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     else:
         out = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, None, kv_len, kv_len, block,
                                                scale)
-    _count(2)
+    _count(2 if q.shape[0] else 0)  # the attention, and the merge of its partial results
     return out
 
 
@@ -207,7 +207,7 @@ def moe_decode(x: torch.Tensor, router: torch.Tensor, w_gate_up, w_down, topk: i
     if isinstance(w_down, torch.Tensor):
         w_down = w_down.unbind(0)
     out = native.lib().moe_decode(x, router, w_gate_up, w_down, topk, residual, out)
-    _count(4)
+    _count(4 if x.shape[0] else 0)  # logits, gate/up, down, combine
     return out
 
 

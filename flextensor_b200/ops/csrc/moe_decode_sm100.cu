@@ -49,6 +49,7 @@ constexpr int MAX_STAGES = 12;
 constexpr int MIN_CHUNKS = 4;           // a CTA takes at least this many weight tiles
 constexpr int TMEM_COLS = 2 * MAX_T;    // two accumulators
 constexpr int RING_BUDGET = 200 * 1024;
+static_assert(MAX_T * MAX_E * 4 <= RING_BUDGET, "the ring holds the logits first");
 
 struct Args {
   int T, D, F, E, topk, slots;          // slots = T * topk (token, choice) pairs
@@ -77,6 +78,7 @@ struct Maps {
   CUtensorMap w[N];
 };
 
+__device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -141,12 +143,12 @@ __global__ void __launch_bounds__(32 * LOGIT_WARPS) moe_logits_kernel(const __gr
 // A token's experts by repeated maximum, by a whole warp: equal logits go to the lower expert, NaN
 // counts as the largest. Lane k < topk gets choice k and its logit.
 template <int PER>  // experts a lane
-__device__ __forceinline__ void choose(const Args& a, int t, int lane, int& mine_e, float& mine) {
+__device__ __forceinline__ void choose(const Args& a, const float* logits, int lane, int& mine_e, float& mine) {
   float v[PER];
   uint32_t key[PER];
 #pragma unroll
   for (int i = 0; i < PER; i++) {
-    v[i] = i * 32 + lane < a.E ? __ldcg(a.logits + t * a.E + i * 32 + lane) : 0.f;
+    v[i] = i * 32 + lane < a.E ? logits[i * 32 + lane] : 0.f;
     const uint32_t b = __float_as_uint(v[i]);
     key[i] = v[i] != v[i] ? 0xffffffffu : (v[i] == 0.f ? 0x80000000u : (b & 0x80000000u ? ~b : b | 0x80000000u));
     if (i * 32 + lane >= a.E) key[i] = 0;  // below every number: -infinity is 0x007fffff
@@ -207,15 +209,20 @@ struct Stream {
   }
 };
 
-// expert tables of every CTA, from the logits
-__device__ void build_tables(Tables& tb, const Args& a, bool keep_weights) {
+// expert tables of every CTA, from the logits, which are brought to shared memory in one go (T * E
+// floats, at most 32 KB of the ring that is still idle): tokens read one after the other from global
+// memory cost 0.8 us each
+__device__ void build_tables(Tables& tb, float* logits, const Args& a, bool keep_weights) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) tb.most = 0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < a.T * a.E; i += NTHREADS) logits[i] = __ldcg(a.logits + i);
+  __syncthreads();
   for (int t = warp; t < a.T; t += NTHREADS / 32) {
     int e;
     float v;
-    if (a.E <= 32) choose<1>(a, t, lane, e, v);
-    else choose<MAX_E / 32>(a, t, lane, e, v);
+    if (a.E <= 32) choose<1>(a, logits + t * a.E, lane, e, v);
+    else choose<MAX_E / 32>(a, logits + t * a.E, lane, e, v);
     if (lane < a.topk) tb.id[t * a.topk + lane] = (short)e;
     if (keep_weights) {  // softmax over the choices; the first is the largest
       const float top = __shfl_sync(0xffffffffu, v, 0);  // by every lane: a shuffle in a branch would wait for the others
@@ -326,7 +333,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
     pdl_wait();
     pdl_launch();
   }
-  build_tables(sm.tb, a, UP && blockIdx.x == 0);
+  build_tables(sm.tb, reinterpret_cast<float*>(ring), a, UP && blockIdx.x == 0);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -353,6 +360,7 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 
   if (warp == 0) {
     if (elect_one()) {
+      fence_proxy_async_shared();  // the ring held the logits
       int s = 0;
       uint32_t ph = 0, pend = 0, pend_ph = 0;
       bool ok = true;
