@@ -140,47 +140,66 @@ __global__ void __launch_bounds__(32 * LOGIT_WARPS) moe_logits_kernel(const __gr
   }
 }
 
-// A token's experts by repeated maximum, by a whole warp: equal logits go to the lower expert, NaN
-// counts as the largest. Lane k < topk gets choice k and its logit.
+// Two tokens' experts by repeated maximum, by a whole warp (two, because each step waits for the one
+// before it): equal logits go to the lower expert, NaN counts as the largest. Lane k < topk gets choice
+// k of each and its logit.
 template <int PER>  // experts a lane
-__device__ __forceinline__ void choose(const Args& a, const float* logits, int lane, int& mine_e, float& mine) {
-  float v[PER];
-  uint32_t key[PER];
+__device__ __forceinline__ void choose(const Args& a, const float* first, const float* second, int lane, int (&mine_e)[2],
+                                       float (&mine)[2]) {
+  float v[2][PER];
+  uint32_t key[2][PER];
 #pragma unroll
-  for (int i = 0; i < PER; i++) {
-    v[i] = i * 32 + lane < a.E ? logits[i * 32 + lane] : 0.f;
-    const uint32_t b = __float_as_uint(v[i]);
-    key[i] = v[i] != v[i] ? 0xffffffffu : (v[i] == 0.f ? 0x80000000u : (b & 0x80000000u ? ~b : b | 0x80000000u));
-    if (i * 32 + lane >= a.E) key[i] = 0;  // below every number: -infinity is 0x007fffff
-  }
-  mine_e = 0;
-  mine = 0.f;
-  for (int k = 0; k < a.topk; k++) {
-    uint32_t best = key[0];
+  for (int n = 0; n < 2; n++) {
 #pragma unroll
-    for (int i = 1; i < PER; i++) best = max(best, key[i]);
-    best = __reduce_max_sync(0xffffffffu, best);
-    unsigned int chosen = 0;
-    float val = 0.f;
-#pragma unroll
-    for (int i = PER - 1; i >= 0; i--) {  // the lowest group that holds it, and its lowest lane
-      const unsigned int m = __ballot_sync(0xffffffffu, key[i] == best);
-      if (m) chosen = i * 32 + __ffs(m) - 1, val = v[i];
+    for (int i = 0; i < PER; i++) {
+      v[n][i] = i * 32 + lane < a.E ? (n ? second : first)[i * 32 + lane] : 0.f;
+      const uint32_t b = __float_as_uint(v[n][i]);
+      key[n][i] = v[n][i] != v[n][i] ? 0xffffffffu : (v[n][i] == 0.f ? 0x80000000u : (b & 0x80000000u ? ~b : b | 0x80000000u));
+      if (i * 32 + lane >= a.E) key[n][i] = 0;  // below every number: -infinity is 0x007fffff
     }
-    val = __shfl_sync(0xffffffffu, val, chosen & 31);
+    mine_e[n] = 0;
+    mine[n] = 0.f;
+  }
+  for (int k = 0; k < a.topk; k++) {
+    uint32_t best[2];
+    int chosen[2];
+    float val[2];
 #pragma unroll
-    for (int i = 0; i < PER; i++)
-      if (i * 32 + lane == chosen) key[i] = 0;
-    if (lane == k) {
-      mine = val;
-      mine_e = (int)chosen;
+    for (int n = 0; n < 2; n++) {
+      best[n] = key[n][0];
+#pragma unroll
+      for (int i = 1; i < PER; i++) best[n] = max(best[n], key[n][i]);
+      best[n] = __reduce_max_sync(0xffffffffu, best[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+      chosen[n] = 0;
+      val[n] = 0.f;
+#pragma unroll
+      for (int i = PER - 1; i >= 0; i--) {  // the lowest group that holds it, and its lowest lane
+        const unsigned int m = __ballot_sync(0xffffffffu, key[n][i] == best[n]);
+        if (m) chosen[n] = i * 32 + __ffs(m) - 1, val[n] = v[n][i];
+      }
+      val[n] = __shfl_sync(0xffffffffu, val[n], chosen[n] & 31);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+#pragma unroll
+      for (int i = 0; i < PER; i++)
+        if (i * 32 + lane == chosen[n]) key[n][i] = 0;
+      if (lane == k) {
+        mine[n] = val[n];
+        mine_e[n] = chosen[n];
+      }
     }
   }
 }
 
 // ------------------------------------------------------------------------------------ the products
 struct Tables {
-  alignas(16) short id[MAX_SLOTS];  // expert of each (token, choice) pair
+  short id[MAX_SLOTS];        // expert of each (token, choice) pair
+  unsigned long long tokens[MAX_E];  // the tokens that chose each expert: a token chooses it once at most
+  int warp_sum[MAX_E / 32];
   short pair[MAX_SLOTS];      // pairs ordered by expert, then token
   short token[MAX_SLOTS];     // and their tokens
   short off[MAX_E + 1];       // first slot of each expert
@@ -214,74 +233,72 @@ struct Stream {
 // memory cost 0.8 us each
 __device__ void build_tables(Tables& tb, float* logits, const Args& a, bool keep_weights) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  static_assert(MAX_T == 64 && NTHREADS >= MAX_E, "a mask holds the tokens, a thread an expert");
   if (threadIdx.x == 0) tb.most = 0;
+  if (threadIdx.x < MAX_E) tb.tokens[threadIdx.x] = 0;
 #pragma unroll 4
   for (int i = threadIdx.x; i < a.T * a.E; i += NTHREADS) logits[i] = __ldcg(a.logits + i);
   __syncthreads();
-  for (int t = warp; t < a.T; t += NTHREADS / 32) {
-    int e;
-    float v;
-    if (a.E <= 32) choose<1>(a, logits + t * a.E, lane, e, v);
-    else choose<MAX_E / 32>(a, logits + t * a.E, lane, e, v);
-    if (lane < a.topk) tb.id[t * a.topk + lane] = (short)e;
-    if (keep_weights) {  // softmax over the choices; the first is the largest
-      const float top = __shfl_sync(0xffffffffu, v, 0);  // by every lane: a shuffle in a branch would wait for the others
-      const float p = lane < a.topk ? expf(v - top) : 0.f;
-      float sum = p;
+  for (int t = warp; t < a.T; t += 2 * (NTHREADS / 32)) {
+    const int u = t + NTHREADS / 32, us = min(u, a.T - 1);  // the second token, if there is one
+    int e[2];
+    float v[2];
+    if (a.E <= 32) choose<1>(a, logits + t * a.E, logits + us * a.E, lane, e, v);
+    else choose<MAX_E / 32>(a, logits + t * a.E, logits + us * a.E, lane, e, v);
 #pragma unroll
-      for (int o = MAX_K / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane < a.topk) a.wts[t * a.topk + lane] = p / sum;
+    for (int n = 0; n < 2; n++) {
+      const int token = n ? u : t;
+      const bool mine = lane < a.topk && token < a.T;
+      if (mine) {
+        tb.id[token * a.topk + lane] = (short)e[n];
+        atomicOr(&tb.tokens[e[n]], 1ull << token);
+      }
+      if (keep_weights) {  // softmax over the choices; the first is the largest
+        const float top = __shfl_sync(0xffffffffu, v[n], 0);  // by every lane: a shuffle in a branch would wait for the others
+        const float p = lane < a.topk ? expf(v[n] - top) : 0.f;
+        float sum = p;
+#pragma unroll
+        for (int o = MAX_K / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (mine) a.wts[token * a.topk + lane] = p / sum;
+      }
     }
   }
-  if (threadIdx.x < 16 && a.slots + threadIdx.x < MAX_SLOTS) tb.id[a.slots + threadIdx.x] = MAX_E;  // no expert
   __syncthreads();
-  // a pair's slot is the number of pairs with a lower expert, or the same one and an earlier place
-  for (int i = threadIdx.x; i < a.slots; i += NTHREADS) {
-    const int e = tb.id[i];
-    int at = 0;
-    for (int j0 = 0; j0 < a.slots; j0 += 8) {
-      const uint4 v = *reinterpret_cast<const uint4*>(tb.id + j0);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  // experts: first slots and the list of the chosen, by a scan over four warps
+  int count = 0, scan = 0;
+  unsigned int used = 0;
+  if (threadIdx.x < MAX_E) {
+    count = __popcll(tb.tokens[threadIdx.x]);  // none for those that do not exist
+    scan = count;
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const int o = (int)(w[k / 2] >> (16 * (k & 1))) & 0xffff;
-        at += o < e || (o == e && j0 + k < i);
-      }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += up;
     }
-    tb.pair[at] = (short)i;
-    tb.token[at] = (short)(i / a.topk);
-  }
-  for (int e0 = 0; e0 < a.E; e0 += NTHREADS) {
-    const int e = e0 + threadIdx.x;
-    int less = 0, same = 0;
-    if (e < a.E) {
-      for (int j0 = 0; j0 < a.slots; j0 += 8) {
-        const uint4 v = *reinterpret_cast<const uint4*>(tb.id + j0);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const int o = (int)(w[k / 2] >> (16 * (k & 1))) & 0xffff;
-          less += o < e;
-          same += o == e;
-        }
-      }
-      tb.off[e] = (short)less;
-      if (e == a.E - 1) tb.off[a.E] = (short)a.slots;
-    }
-    const unsigned int m = __ballot_sync(0xffffffffu, same > 0);
-    const int most = __reduce_max_sync(0xffffffffu, same);
-    if (lane == 0 && e / 32 < MAX_E / 32) {
-      tb.used[e / 32] = m;
+    used = __ballot_sync(0xffffffffu, count > 0);
+    const int most = __reduce_max_sync(0xffffffffu, count);
+    if (lane == 31) tb.warp_sum[warp] = scan;
+    if (lane == 0) {
+      tb.used[warp] = used;
       atomicMax(&tb.most, most);
     }
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.E; e += NTHREADS) {
-    int at = __popc(tb.used[e / 32] & ((1u << (e % 32)) - 1));
-    for (int i = 0; i < e / 32; i++) at += __popc(tb.used[i]);
-    const bool here = tb.used[e / 32] >> (e % 32) & 1;
-    if (here) tb.act[at] = (short)e;
-    if (e == a.E - 1) tb.n_act = at + here;
+  if (threadIdx.x < MAX_E) {
+    int off = scan - count, at = __popc(used & ((1u << lane) - 1));
+    for (int w = 0; w < warp; w++) off += tb.warp_sum[w], at += __popc(tb.used[w]);
+    tb.off[threadIdx.x] = (short)off;
+    if (count > 0) tb.act[at] = (short)threadIdx.x;
+    if (threadIdx.x == MAX_E - 1) {
+      tb.off[MAX_E] = (short)a.slots;
+      tb.n_act = at + (count > 0);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.slots; i += NTHREADS) {  // a pair's slot: its expert's first, and the earlier tokens there
+    const int e = tb.id[i], t = i / a.topk, at = tb.off[e] + __popcll(tb.tokens[e] & ((1ull << t) - 1));
+    tb.pair[at] = (short)i;
+    tb.token[at] = (short)t;
   }
   __syncthreads();
 }
@@ -351,8 +368,8 @@ __global__ void __launch_bounds__(NTHREADS, 1)
   if (UP && cta == 0) {  // where each pair's row of h and of the partial sums is, for the combine kernel
     for (int s = threadIdx.x; s < a.slots; s += NTHREADS) {
       const int e = tb.id[tb.pair[s]];
-      int ai = 0;  // its place among the chosen experts
-      while (tb.act[ai] != e) ai++;
+      int ai = __popc(tb.used[e / 32] & ((1u << (e % 32)) - 1));  // its place among the chosen experts
+      for (int w = 0; w < e / 32; w++) ai += __popc(tb.used[w]);
       a.place[tb.pair[s]] = s | ai << 16;
     }
     if (threadIdx.x == 0) a.place[a.slots] = tb.n_act;
