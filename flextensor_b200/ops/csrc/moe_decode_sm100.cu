@@ -577,13 +577,22 @@ __global__ void __launch_bounds__(NTHREADS, 1)
           }
           asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");
           if (sm.last) {
-            constexpr int COLS = 4;  // columns in flight
+            constexpr int COLS = 8;  // columns in flight, of two runs
             for (int j0 = 0; j0 < n; j0 += COLS) {
               float v[COLS] = {};
-              for (int c = c0; c <= c1; c++) {
-                const float* const from = tile(c);
+              for (int c = c0; c <= c1; c += 2) {
+                const float *const from = tile(c), *const next = tile(min(c + 1, c1));
+                float x[COLS], y[COLS];
 #pragma unroll
-                for (int u = 0; u < COLS; u++) v[u] += __ldcg(from + (long long)min(j0 + u, n - 1) * BM);
+                for (int u = 0; u < COLS; u++) {
+                  x[u] = __ldcg(from + (long long)min(j0 + u, n - 1) * BM);
+                  y[u] = __ldcg(next + (long long)min(j0 + u, n - 1) * BM);
+                }
+#pragma unroll
+                for (int u = 0; u < COLS; u++) {
+                  v[u] += x[u];
+                  if (c < c1) v[u] += y[u];
+                }
               }
 #pragma unroll
               for (int u = 0; u < COLS; u++)
