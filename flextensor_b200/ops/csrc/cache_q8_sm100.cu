@@ -568,22 +568,30 @@ struct Runs {
 };
 
 // A warp's place in its CTA's run: a tile of units [t, min(t + units of a tile, end)) of a piece, the
-// run's part of one step of heads of one sequence.
+// run's part of one step of heads of one sequence. The tiles of a piece go to the warps of a head in
+// turn, beginning with the one after the piece before: tile i of a piece is warp (i + turn) % keys'.
 struct Cursor {
-  int b, j, t, end, left;  // sequence, step of heads, first unit, end of the piece, places of the run after the piece
+  int b, j, t, from, end, left;  // sequence, step of heads, unit, the piece's units [from, end), places of the run after it
+  int turn;
 
-  // the tile `step` units further on, `start` units into a piece where that leaves this one; false at the run's end
-  __device__ __forceinline__ bool next(const DecArgs& a, int step, int start) {
-    t += step;
+  // this warp's place in the turn, which numbers its partial result of the piece
+  __device__ __forceinline__ int key(const DecArgs& a, int warp_key) const { return (warp_key - turn) & (a.keys - 1); }
+
+  // this warp's next tile (its first where t is the piece's begin and `first`); false at the run's end
+  template <int UT>
+  __device__ __forceinline__ bool next(const DecArgs& a, int warp_key, bool first) {
+    t += first ? key(a, warp_key) * UT : a.keys * UT;
     while (t >= end) {
       if (left == 0) return false;
+      turn += max(0, (end - from + UT - 1) / UT);
       int n = 0;
       if (++j == a.per) j = 0, b++;
       while ((n = seq_cost(a, b)) == 0) b++;  // places are left, so a sequence with some follows
       n = min(n, left);
       left -= n;
+      from = 0;
       end = n - ENTRY;
-      t = start;
+      t = key(a, warp_key) * UT;
     }
     return true;
   }
@@ -621,7 +629,8 @@ __device__ __forceinline__ Cursor locate(const DecArgs& a, int i, int count, int
   c.j = i / n;
   i -= c.j * n;
   c.left = count - (min(n, i + count) - i);
-  c.t = max(0, i - ENTRY);
+  c.from = c.t = max(0, i - ENTRY);
+  c.turn = 0;
   c.end = min(n, i + count) - ENTRY;
   return c;
 }
@@ -685,9 +694,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
   const int run = blockIdx.x;
   if (run >= runs.n) return;
   const int first = runs.begin(run), count = runs.begin(run + 1) - first;
-  const int my_head = warp % a.heads, start = warp / a.heads * UT, step = a.keys * UT;
+  const int my_head = warp % a.heads, my_key = warp / a.heads;
   Cursor at = locate(a, first, count, lane);
-  if (!at.next(a, start, start)) return;  // a run too short for this warp
+  if (!at.next<UT>(a, my_key, true)) return;  // a run too short for this warp
   Cursor ahead = at;
   auto fetch = [&](int s, bool values) {  // keys or values of the tile at `ahead` into slot s
     if (lane == 0) {
@@ -754,7 +763,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
   prepare(at);  // before the copies: behind 192 KB an SM of them these loads took 5 us
   fetch(0, false);
   fetch(1, true);
-  bool more = ahead.next(a, step, start);  // whether `ahead` is a tile after `at`
+  bool more = ahead.next<UT>(a, my_key, false);  // whether `ahead` is a tile after `at`
   if (more) fetch(2, false);
   enter();
   bool ok = true;
@@ -802,7 +811,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
     }
     if (last) {
       // step of heads + run grows from one piece to the next: it numbers the pieces
-      const long long piece = ((long long)at.b * a.per + at.j + run) * WARPS + warp;
+      const long long piece = ((long long)at.b * a.per + at.j + run) * WARPS + at.key(a, my_key) * a.heads + my_head;
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -823,7 +832,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
     }
     if (!more) break;
     at = ahead;
-    more = ahead.next(a, step, start);
+    more = ahead.next<UT>(a, my_key, false);
     if (more && ok) fetch(s, false);
     turn();
     if (last) enter();
@@ -866,7 +875,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(const __g
       const int cnt = (runs.owner(f + n - 1) + 1 - r0) * a.keys;
       lo = cnt * part / per;
       hi = cnt * (part + 1) / per;
-      // partial i: run r0 + i / keys, the warp of this head with key tiles i % keys
+      // partial i: run r0 + i / keys, the warp of this head that is i % keys in turn
       base = (((long long)b * a.per + j + r0) * WARPS + hg - j * a.heads) * (8 * NT) + r % (8 * NT);
       stride = a.heads * 8 * NT;
     }

@@ -40,7 +40,7 @@ def taken(lens, heads_groups, ut, sms):
     for run in range(runs.n):
         first, count = runs.begin(run), runs.begin(run + 1) - runs.begin(run)
         for warp in range(WARPS):
-            my_head, start, step = warp % heads, warp // heads * ut, keys * ut
+            my_head, my_key, turn = warp % heads, warp // heads, 0
             # locate
             i, b = first, 0
             while i >= cost[b] * per:
@@ -49,13 +49,15 @@ def taken(lens, heads_groups, ut, sms):
             n = cost[b]
             j, i = divmod(i, n)
             left = count - (min(n, i + count) - i)
-            t, end = max(0, i - ENTRY) + start, min(n, i + count) - ENTRY
+            start, end = max(0, i - ENTRY), min(n, i + count) - ENTRY
+            t = start + my_key * ut
             while True:
                 done = False
                 while t >= end:
                     if left == 0:
                         done = True
                         break
+                    turn += max(0, -(-(end - start) // ut))
                     j += 1
                     if j == per:
                         j, b = 0, b + 1
@@ -63,20 +65,21 @@ def taken(lens, heads_groups, ut, sms):
                         b += 1
                     n = min(cost[b], left)
                     left -= n
-                    end, t = n - ENTRY, start
+                    start, end = 0, n - ENTRY
+                    t = (my_key - turn) % keys * ut
                 if done:
                     break
                 hg = j * heads + my_head
                 for u in range(t, min(t + ut, end)):
                     d = got.setdefault((b, hg), {})
                     d[u] = d.get(u, 0) + 1
-                key = (run, warp // heads)
+                key = (run, (my_key - turn) % keys)
                 if key not in partials.setdefault((b, hg), []):
                     partials[b, hg].append(key)
-                    number = (b * per + j + run) * WARPS + warp
+                    number = (b * per + j + run) * WARPS + key[1] * heads + my_head
                     assert number not in seen
                     seen.add(number)
-                t += step
+                t += keys * ut
     assert not seen or max(seen) < (len(lens) * per + sms) * WARPS
     return got, partials
 
