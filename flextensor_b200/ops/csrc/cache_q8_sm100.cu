@@ -277,6 +277,11 @@ __device__ __forceinline__ float lg2f(float x) {
   return y;
 }
 
+// 2^(d/2) for a difference of references d down to -252: sums are scaled by it twice. A block of zeros puts
+// its reference up to 181 below that of values beside it while its keys' p are as large, and 2^d by itself
+// would be 0 there; for the outputs, which are in the unit of the reference, that is right.
+__device__ __forceinline__ float root_of_scale(float d) { return ex2f(0.5f * d); }
+
 // maximum that keeps a NaN (fmaxf drops it): a NaN score has to reach its row's output
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
@@ -396,8 +401,15 @@ struct RowState {
   float m[NT][2], l[NT][2];
 };
 
-// The scales of a tile's 16-key groups: keys' scale, values' scale, its log2 (the reference of the
-// weights) and its inverse. A group whose scale is not an ordinary number gets a weight of its own.
+// The scales of a tile's 16-key groups, keys' and values'.
+// In the reference a value scale counts as at least 2^-60 and at most 2^121 (the largest that bf16 values
+// give), so a key's p is at most 2^75 (blocks of zeros) and at least 2^-114 where it weighs most. Tiles with
+// a scale outside 2^+-30 compute p by itself, the others as (p * vs) / vs, which has fp32's precision beside
+// value scales up to 2^90 times larger. Values of scales below 2^-84 underflow to 0.
+constexpr float V_SCALE_MIN = 0x1p-60f, V_SCALE_MAX = 0x1p121f, V_SCALE_ODD = 0x1p30f;
+// The sums of p are kept 2^20 times larger: between 2^-94 and, over 2^32 keys, 2^127.
+constexpr float SUM_UNIT = 0x1p20f;
+
 template <int MT>
 struct TileScales {
   float k[MT], v[MT];
@@ -440,13 +452,13 @@ __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT
   }
   keys_read();
   float lv[MT], iv[MT];
-  bool odd = false;  // a value scale that is 0, tiny, huge or NaN
+  bool odd = false;  // a value scale that is 0, small, large or NaN
 #pragma unroll
   for (int mt = 0; mt < MT; mt++) {
-    odd |= !(sc.v[mt] >= 0x1p-100f && sc.v[mt] <= 0x1p100f);
-    const float v = fminf(fmaxf(sc.v[mt], 0x1p-100f), 0x1p100f);
+    odd |= !(sc.v[mt] >= 1.f / V_SCALE_ODD && sc.v[mt] <= V_SCALE_ODD);
+    const float v = fminf(fmaxf(sc.v[mt], V_SCALE_MIN), V_SCALE_MAX);
     lv[mt] = lg2f(v);
-    iv[mt] = __fdividef(1.f, v);
+    iv[mt] = __fdividef(SUM_UNIT, v);
   }
   uint32_t pb[MT][NT][2];
 #pragma unroll
@@ -483,9 +495,9 @@ __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT
         top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 8));
         top[i] = max_nan(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
         const float m_new = max_nan(st.m[nt][i], top[i] - 7.f);
-        const float al = st.m[nt][i] == -INFINITY ? 0.f : ex2f(st.m[nt][i] - m_new);
+        const float root = st.m[nt][i] == -INFINITY ? 0.f : root_of_scale(st.m[nt][i] - m_new), al = root * root;
         st.m[nt][i] = m_new;
-        st.l[nt][i] *= al;
+        st.l[nt][i] = st.l[nt][i] * root * root;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
           st.o[j][nt][i] *= al;
@@ -494,20 +506,32 @@ __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT
       }
     }
     const float ref[2] = {st.m[nt][0] == -INFINITY ? 0.f : st.m[nt][0], st.m[nt][1] == -INFINITY ? 0.f : st.m[nt][1]};
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-      const float d0 = lv[mt] - ref[0], d1 = lv[mt] - ref[1];
-      float w[4] = {ex2f(s[mt][nt][0] + d0), ex2f(s[mt][nt][1] + d1), ex2f(s[mt][nt][2] + d0), ex2f(s[mt][nt][3] + d1)};
-      st.l[nt][0] = fmaf(w[0] + w[2], iv[mt], st.l[nt][0]);
-      st.l[nt][1] = fmaf(w[1] + w[3], iv[mt], st.l[nt][1]);
-      if (odd) {  // the weight is p * vs: 0 for a scale of 0, NaN for NaN, and 0 for what the column does not see
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          w[e] = masked && mt * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1] ? 0.f : w[e] * iv[mt] * sc.v[mt];
-      }
-      __half2 h0 = __floats2half2_rn(w[0], w[1]), h1 = __floats2half2_rn(w[2], w[3]);
+    auto weights = [&](int mt, float w0, float w1, float w2, float w3) {
+      __half2 h0 = __floats2half2_rn(w0, w1), h1 = __floats2half2_rn(w2, w3);
       pb[mt][nt][0] = transpose8x8(*reinterpret_cast<uint32_t*>(&h0));
       pb[mt][nt][1] = transpose8x8(*reinterpret_cast<uint32_t*>(&h1));
+    };
+    if (!odd) {  // two loops: a branch inside one kept scores alive and cost 2 us of 53
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++) {
+        const float d0 = lv[mt] - ref[0], d1 = lv[mt] - ref[1];
+        const float w[4] = {ex2f(s[mt][nt][0] + d0), ex2f(s[mt][nt][1] + d1), ex2f(s[mt][nt][2] + d0), ex2f(s[mt][nt][3] + d1)};
+        st.l[nt][0] = fmaf(w[0] + w[2], iv[mt], st.l[nt][0]);
+        st.l[nt][1] = fmaf(w[1] + w[3], iv[mt], st.l[nt][1]);
+        weights(mt, w[0], w[1], w[2], w[3]);
+      }
+    } else {  // p * vs is 0 for a scale of 0, NaN for NaN, and 0 for what the column does not see
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float p = ex2f(s[mt][nt][e] - ref[e & 1]);
+          st.l[nt][e & 1] = fmaf(p, SUM_UNIT, st.l[nt][e & 1]);
+          w[e] = masked && mt * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1] ? 0.f : p * sc.v[mt];
+        }
+        weights(mt, w[0], w[1], w[2], w[3]);
+      }
     }
   }
   if (!values_here()) return;
@@ -668,8 +692,8 @@ struct DecSmem {
   uint64_t full[WARPS][SLOTS];
 };
 
-// Bound by HBM where sequences are long (131071 tokens, 8 heads, e4m3: 268 MB in 49 us with the merge,
-// 5.4 TB/s; 32 x 2304 tokens, int8: 151 MB in 36 us, of which 24 us stream) and by latency where they
+// Bound by HBM where sequences are long (131071 tokens, 8 heads, e4m3: 268 MB in 53 us with the merge,
+// 5.1 TB/s; 32 x 2304 tokens, int8: 152 MB in 35 us, of which 24 us stream) and by latency where they
 // are short. The loads of a head's queries and scales come before the copies, which would hold them
 // up for 5 us in the memory's queues.
 template <int NT, int FMT>
@@ -900,18 +924,20 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(const __g
     for (int o = 4; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     top = __shfl_sync(0xffffffffu, top, 0);
     const float m_new = max_nan(M, top), ref = m_new == -INFINITY ? 0.f : m_new;
-    const float al = M == -INFINITY ? 0.f : ex2f(M - ref), w = ml.x == -INFINITY ? 0.f : ex2f(ml.x - ref);
+    const float root = M == -INFINITY ? 0.f : root_of_scale(M - ref), al = root * root;
+    const bool none = ml.x == -INFINITY;  // nothing was written there, or nothing of it counts
+    const float wr = root_of_scale(ml.x - ref), w = none ? -1.f : wr * wr, lw = none ? 0.f : ml.y * wr * wr;
+    L = L * root * root;
     M = m_new;
-    L *= al;
     acc.x *= al;
     acc.y *= al;
     acc.z *= al;
     acc.w *= al;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float wi = __shfl_sync(0xffffffffu, w, i), li = __shfl_sync(0xffffffffu, ml.y, i);
-      if (wi == 0.f) continue;  // nothing was written there, or nothing of it counts
-      L = fmaf(wi, li, L);
+      const float wi = __shfl_sync(0xffffffffu, w, i), li = __shfl_sync(0xffffffffu, lw, i);
+      if (wi < 0.f) continue;
+      L += li;
       acc.x = fmaf(wi, v[i].x, acc.x);
       acc.y = fmaf(wi, v[i].y, acc.y);
       acc.z = fmaf(wi, v[i].z, acc.z);
@@ -929,18 +955,20 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(const __g
     acc = make_float4(0.f, 0.f, 0.f, 0.f);
     L = 0.f;
     for (int i = 0; i < per; i++) {
-      const float w = sml[warp + i].x == -INFINITY ? 0.f : ex2f(sml[warp + i].x - ref);
+      if (sml[warp + i].x == -INFINITY) continue;
+      const float wr = root_of_scale(sml[warp + i].x - ref), w = wr * wr;
       const float4 v = so[warp + i][lane];
       acc.x = fmaf(w, v.x, acc.x);
       acc.y = fmaf(w, v.y, acc.y);
       acc.z = fmaf(w, v.z, acc.z);
       acc.w = fmaf(w, v.w, acc.w);
-      L += w * sml[warp + i].y;
+      L += sml[warp + i].y * wr * wr;
     }
   }
   if (row >= rows) return;
   const float inv = 1.f / L;
-  uint2 out = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  uint2 out = make_uint2(pack_bf16x2(acc.x * SUM_UNIT * inv, acc.y * SUM_UNIT * inv),
+                         pack_bf16x2(acc.z * SUM_UNIT * inv, acc.w * SUM_UNIT * inv));
   if (len - a.Sq + 1 + r / a.G <= 0) out = make_uint2(0, 0);  // the row sees no key
   *reinterpret_cast<uint2*>(a.o + b * a.o_b + (long long)(r / a.G) * a.o_tok + (long long)(h * a.G + r % a.G) * a.o_h + 4 * lane) = out;
 }

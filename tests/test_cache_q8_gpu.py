@@ -264,6 +264,34 @@ def test_attention_scales_and_magnitudes():
     check_attend((q.float() * 2.0 ** -108).bfloat16(), cache, [L], block, L)
 
 
+@pytest.mark.parametrize("scale", [2.0 ** 115, 2.0 ** 60, 2.0 ** -70])
+def test_attention_far_value_scales(scale):
+    """All values huge or tiny, a third of them zero up to 2^60 (their sum and the zeros' are far apart in size)."""
+    L, block = 384, 32
+    cache = junk_cache("int8", 2, L, 2, block, 41)
+    cache[3].fill_(scale)
+    if scale == 2.0 ** 60:
+        cache[3][:, ::3] = 0
+    check_attend(bf16(42, 2, 8, 128, spread=False), cache, [L, 200], block, torch.tensor([L, 200], dtype=torch.int32, device=DEV))
+
+
+def test_attention_zeros_before_values():
+    """12288 keys with zero values, all but the first of them e^5.5 heavier, then 4096 with values: the
+    zeros only divide. One warp passes over a whole sequence here (more sequences than SMs)."""
+    B, L, Hk, block = 160, 16384, 8, 64
+    one = new_cache("int8", 1, L, Hk, block)
+    one[0][:, block:, :, 0] = 64
+    one[1][:, 12288:] = 64
+    one[2].fill_(2.0 ** -6)
+    one[3][:, 12288 // block:] = 2.0 ** -6
+    q = torch.zeros(B, Hk, 128, device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = 5.5 * 128 ** 0.5
+    got = ops.decode_attention_q8(q, *[c.expand(B, *c.shape[1:]) for c in one], L, block=block)
+    torch.cuda.synchronize()
+    want, A = ref_attend(q[:1, None], one, [L], block)
+    assert bool(((got.double() - want[0]).abs() <= want[0].abs() * 2 ** -8 + A[0] * 2 ** -9).all())
+
+
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_attention_many_small_weights(fmt):
     """One key outweighs each of 131071 others by e^18 = 2^26, and its value is zero: the output is what
