@@ -39,4 +39,5 @@ for ((r = 0; r < REPLICAS; r++)); do
   pids+=($!)
 done
 trap 'kill "${pids[@]}" 2>/dev/null || true' EXIT INT TERM
+sleep 1  # an nginx that ends at once (its port taken) ends the replicas: let them start, so that each has said so
 nginx -c "$HERE/nginx.conf" -g "daemon off;"
