@@ -172,7 +172,8 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                         max_len: int | None = None, scale: float | None = None,
                         out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`decode_attention` over a cache written by :func:`kv_append_q8` (or any codes with
-    scales that are not negative; e4m3 codes must be finite).
+    scales that are not negative; e4m3 codes must be finite; value scales below 2**-84 count as 0, and
+    a sequence's others should lie within 2**90 of one another).
 
     ``q [B, Hq, 128]``, or ``[B, Sq, Hq, 128]`` for the last Sq tokens of each sequence, whose keys
     are in the cache already (a few: the workspace grows with Sq): query i sees keys ``[0, kv_len - Sq + 1 + i)``; one that sees none
