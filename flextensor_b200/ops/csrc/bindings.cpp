@@ -462,6 +462,8 @@ Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tenso
   TORCH_CHECK(D >= 8 && D % 8 == 0 && F >= 8 && F % 8 == 0 && D < (1 << 20) && F < (1 << 20), op,
               ": D and F must be multiples of 8, got ", D, " and ", F);
   matrix(x, "x", T, D);
+  // tensor maps take no repeated rows
+  TORCH_CHECK(T <= 1 || x.stride(0) >= D, op, ": rows of x must not overlap");
   matrix(router, "router", E, D);
   const Tensor out = out_given && out_given->defined() ? *out_given
                      : x.is_cuda() ? Tensor(at::detail::empty_cuda({T, D}, at::kBFloat16, x.device(), c10::nullopt))
@@ -478,6 +480,7 @@ Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tenso
       if (t.scalar_type() != at::kBFloat16 || size.size() != 2 || size[0] != r || size[1] != c || stride[1] != 1 ||
           stride[0] % 8 != 0 || !on_16_bytes(t))
         matrix(t, name, r, c);
+      TORCH_CHECK(stride[0] >= c, op, ": rows of ", name, " must not overlap");
       TORCH_CHECK(stride[0] == w[0].stride(0), op, ": the experts' weights must have one row stride");
       to[e] = reinterpret_cast<const __nv_bfloat16*>(t.const_data_ptr());
     }
@@ -498,7 +501,7 @@ Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tenso
   p.E = (int)E;
   p.topk = (int)topk;
   p.x = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
-  p.ldx = x.stride(0);
+  p.ldx = T == 1 ? D : x.stride(0);
   p.router = reinterpret_cast<const __nv_bfloat16*>(router.data_ptr());
   p.ldr = router.stride(0);
   p.ld_gate_up = gate_up[0].stride(0);
@@ -875,7 +878,8 @@ int device_error(bool reset) {
   int m = ft::moe_device_error(reset);
   int d = ft::decode_device_error(reset);
   int c = ft::cache_device_error(reset);
-  return e ? e : (n ? n : (a ? a : (p ? p : (t ? t : (m ? m : (d ? d : (c ? c : ft::moe_decode_device_error(reset))))))));
+  int o = ft::moe_decode_device_error(reset);
+  return e ? e : (n ? n : (a ? a : (p ? p : (t ? t : (m ? m : (d ? d : (c ? c : o)))))));
 }
 
 struct PyEngine {

@@ -40,6 +40,8 @@ def bf(*s):
     (dict(residual=bf(T, D + 8)), "residual must be"),
     (dict(out=bf(T + 1, D)), "out must be"),
     (dict(out=bf(1, D).expand(T, D)), "overlap"),
+    (dict(x=bf(1, D).expand(T, D)), "rows of x must not overlap"),
+    (dict(w_down=[bf(1, F).expand(D, F)] * 4), "rows of w_down must not overlap"),
 ])
 def test_refusals(change, match):
     a = args()

@@ -85,6 +85,8 @@ def test_strides_and_aliases():
     assert torch.equal(ops.moe_decode(**dict(p, x=x), topk=2, residual=res, out=x), want)
     one = torch.zeros(1, 256, device=DEV, dtype=torch.bfloat16).expand(9, 256)
     assert torch.equal(ops.moe_decode(**p, topk=2, residual=one), ops.moe_decode(**p, topk=2))
+    single = dict(p, x=p["x"][:1])  # a single row may have any row stride
+    assert torch.equal(ops.moe_decode(**dict(p, x=p["x"].as_strided((1, 256), (0, 1))), topk=2), check(single, 2))
 
 
 def test_shared_and_scattered_experts():
