@@ -164,7 +164,7 @@ def kv_append_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
         native.lib().kv_append_q8(k, v, k_cache, v_cache, k_scale, v_scale, pos, 0, n_new, block)
     else:
         native.lib().kv_append_q8(k, v, k_cache, v_cache, k_scale, v_scale, None, pos, n_new, block)
-    _count(1 if k.shape[1] else 0)
+    _count(1 if k.numel() else 0)
 
 
 def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
@@ -185,9 +185,11 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
         ml = k_cache.shape[1] if max_len is None else max_len
         out = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, kv_len, 0, ml, block, scale)
     else:
+        ml = kv_len
         out = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, None, kv_len, kv_len, block,
                                                scale)
-    _count(2 if q.shape[0] else 0)  # the attention, and the merge of its partial results
+    if q.numel():
+        _count(2 if ml > 0 else 1)  # the attention, if there are keys, and the merge of its partial results
     return out
 
 

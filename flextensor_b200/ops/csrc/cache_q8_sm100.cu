@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(const __g
   float M = -INFINITY, L = 0.f;
   int r = 0, h = 0, b = 0, len = 0;
   // The lengths are there: this kernel starts only after every CTA of the first one has waited for what
-  // was before it.
+  // was before it. (Without a first one no key may count, whatever they are.)
   int r0 = 0, lo = 0, hi = 0, f = 0, n = 0, stride = 0;
   long long base = 0;
   Runs runs(0, 0);
@@ -1007,9 +1007,11 @@ cudaError_t launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const De
     if (err == cudaSuccess && dev < 64) ready[dev] = true;
   }
   if (err != cudaSuccess) return err;
-  const cudaError_t e =
-      launch_overlapped(cache_decode_kernel<NT, FMT>, (unsigned)sms, 32 * WARPS, smem, stream, tk, tv, a);
-  if (e != cudaSuccess) return e;
+  return launch_overlapped(cache_decode_kernel<NT, FMT>, (unsigned)sms, 32 * WARPS, smem, stream, tk, tv, a);
+}
+
+template <int NT>
+cudaError_t launch_merge(const DecArgs& a, cudaStream_t stream) {
   // CTAs of four warps, or of one row's where that is more: small ones fill the SMs evenly
   const int warps = std::max(4, a.merge_per_row), rows_here = warps / a.merge_per_row;
   const int rows = a.B * a.Hk * a.R;
@@ -1089,13 +1091,18 @@ cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream) {
   // a row has at most about this many partials; warps that share it take a few each
   const long long expect = (a.runs / head_steps_of(p) + 1) * a.keys;
   a.merge_per_row = expect >= 64 ? 16 : expect >= 32 ? 8 : expect >= 16 ? 4 : expect >= 8 ? 2 : 1;
-  CUtensorMap tk, tv;
-  if (p.L > 0 && (!side_map(&tk, p.side[0], p, a.one_b[0], a.one_h[0]) || !side_map(&tv, p.side[1], p, a.one_b[1], a.one_h[1])))
-    return cudaErrorInvalidValue;
-  const bool i8 = p.format == CACHE_INT8;
-  if (col_tiles(p) == 1)
-    return i8 ? launch_decode<1, CACHE_INT8>(tk, tv, a, p.num_sms, stream) : launch_decode<1, CACHE_E4M3>(tk, tv, a, p.num_sms, stream);
-  return i8 ? launch_decode<2, CACHE_INT8>(tk, tv, a, p.num_sms, stream) : launch_decode<2, CACHE_E4M3>(tk, tv, a, p.num_sms, stream);
+  const bool one = col_tiles(p) == 1;
+  if (p.max_len > 0) {  // without keys there may be no memory to map; the merge alone writes the zeros
+    CUtensorMap tk, tv;
+    if (!side_map(&tk, p.side[0], p, a.one_b[0], a.one_h[0]) || !side_map(&tv, p.side[1], p, a.one_b[1], a.one_h[1]))
+      return cudaErrorInvalidValue;
+    const bool i8 = p.format == CACHE_INT8;
+    const cudaError_t e =
+        one ? (i8 ? launch_decode<1, CACHE_INT8>(tk, tv, a, p.num_sms, stream) : launch_decode<1, CACHE_E4M3>(tk, tv, a, p.num_sms, stream))
+            : (i8 ? launch_decode<2, CACHE_INT8>(tk, tv, a, p.num_sms, stream) : launch_decode<2, CACHE_E4M3>(tk, tv, a, p.num_sms, stream));
+    if (e != cudaSuccess) return e;
+  }
+  return one ? launch_merge<1>(a, stream) : launch_merge<2>(a, stream);
 }
 
 }  // namespace ft

@@ -43,7 +43,7 @@ struct CacheDecodeProblem {
   float* scratch = nullptr;                // cache_decode_scratch_floats(p) floats
 };
 size_t cache_decode_scratch_floats(const CacheDecodeProblem& p);
-// two kernels
+// two kernels; where max_len is 0, the second alone
 cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream);
 int cache_device_error(bool reset);
 

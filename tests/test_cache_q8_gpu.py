@@ -402,3 +402,16 @@ def test_empty_calls():
     assert bool((ops.decode_attention_q8(bf16(1, 2, 4, 128, spread=False), *cache, 0) == 0).all())
     none = junk_cache("int8", 1, 0, 2, 64, 13)
     assert bool((ops.decode_attention_q8(bf16(1, 1, 4, 128, spread=False), *none, 0) == 0).all())
+
+
+def test_attention_without_keys_takes_the_merge_alone():
+    """No key may count (a cache of length 0, or max_len 0): no tensor map is made of it and the first
+    kernel is not launched; the lengths on the device have no say."""
+    q = bf16(1, 1, 3, 4, 128, spread=False)
+    for L, kv_len in ((0, 0), (0, torch.tensor([7], dtype=torch.int32, device=DEV)), (40, 0),
+                      (40, torch.tensor([40], dtype=torch.int32, device=DEV))):
+        cache = junk_cache("int8", 1, L, 2, 64, 13)
+        before = ops.launch_count()
+        got = ops.decode_attention_q8(q, *cache, kv_len, max_len=0, out=torch.full_like(q, 7.0))
+        assert ops.launch_count() - before == 1 and bool((got == 0).all())
+    assert native.device_error(reset=True) == 0
