@@ -415,3 +415,60 @@ def test_attention_without_keys_takes_the_merge_alone():
         got = ops.decode_attention_q8(q, *cache, kv_len, max_len=0, out=torch.full_like(q, 7.0))
         assert ops.launch_count() - before == 1 and bool((got == 0).all())
     assert native.device_error(reset=True) == 0
+
+
+@pytest.mark.parametrize("scale,top", [(2.0 ** 121, 60), (2.0 ** 122, 60), (2.0 ** 126, 3), (2.0 ** 127, 1)])
+def test_attention_largest_value_scales(scale, top):
+    """The largest scales that the append makes (2^122: int8 codes of bf16's largest values) and larger
+    ones. 64 keys of weight 1, then 64 of up to 2^8: a weight of the second tile is as far above the first
+    tile's reference as it may be without moving it. More sequences than SMs, so that a warp passes over
+    both tiles."""
+    B, L, Hk, block = 160, 128, 8, 64
+    g = torch.Generator(device=DEV).manual_seed(3)
+    one = new_cache("int8", 1, L, Hk, block)
+    one[0][:, block:, :, 0] = 64
+    one[1].copy_(torch.randint(-top, top + 1, one[1].shape, device=DEV, generator=g))
+    one[2].fill_(2.0 ** -6)
+    one[3].fill_(scale)
+    q = torch.zeros(B, Hk, 128, device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = torch.tensor([8.0, 7.96875, 7.5, 6.0, 4.0, 2.0, 0.0, -8.0], device=DEV)
+    ln2 = 0.6931471805599453  # scores in units of log2
+    got = ops.decode_attention_q8(q, *[c.expand(B, *c.shape[1:]) for c in one], L, block=block, scale=ln2)
+    torch.cuda.synchronize()
+    want, A = ref_attend((q[:1, None].double() * (ln2 * 128 ** 0.5)), one, [L], block)
+    assert bool(((got.double() - want[0]).abs() <= want[0].abs() * 2 ** -8 + A[0] * 2 ** -9).all())
+    assert native.device_error(reset=True) == 0
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** 100, 2.0 ** 121, 2.0 ** 126])
+def test_attention_small_weights_of_large_values(scale):
+    """16383 keys, each 2^18 lighter than the first, whose value is zero: together 1/16 of its weight, at any
+    size of the values. One warp passes over a whole sequence (more sequences than SMs)."""
+    B, L, Hk, block = 160, 16384, 8, 64
+    one = new_cache("int8", 1, L, Hk, block)
+    one[0][:, 0, :, 0] = 64
+    one[1][:, 1:] = 3
+    one[2].fill_(2.0 ** -6)
+    one[3].fill_(scale)
+    q = torch.zeros(B, Hk, 128, device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = 18.0
+    ln2 = 0.6931471805599453
+    got = ops.decode_attention_q8(q, *[c.expand(B, *c.shape[1:]) for c in one], L, block=block, scale=ln2)
+    torch.cuda.synchronize()
+    want, A = ref_attend((q[:1, None].double() * (ln2 * 128 ** 0.5)), one, [L], block)
+    assert float(want.min()) > 0.17 * scale
+    assert bool(((got.double() - want[0]).abs() <= want[0].abs() * 2 ** -8 + A[0] * 2 ** -9).all())
+
+
+def test_attention_infinite_value_scales_stay():
+    """A block of an infinite value scale makes the rows that see it infinite or NaN and no others."""
+    B, Sq, L, Hk, block = 1, 2, 96, 1, 16
+    cache = junk_cache("int8", B, L, Hk, block, 43)
+    cache[1][:, 48:64] = 1
+    cache[3][0, 3] = float("inf")
+    q = bf16(44, B, Sq, 4, 128, spread=False)
+    clean = [c.clone() for c in cache]
+    clean[3][0, 3] = 0
+    n = torch.tensor([49], dtype=torch.int32, device=DEV)  # query 0 sees 48 keys, none of block 3
+    got = ops.decode_attention_q8(q, *cache, n, block=block)
+    assert torch.equal(got[:, :1], ops.decode_attention_q8(q, *clean, n, block=block)[:, :1]) and not got[:, 1:].isfinite().any()
