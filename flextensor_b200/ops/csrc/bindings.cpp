@@ -9,7 +9,11 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cstdlib>
+#include <functional>
+#include <utility>
+#include <vector>
 
 #include "ft_attn.h"
 #include "ft_cache.h"
@@ -327,6 +331,32 @@ void check_rows(const Tensor& t, const char* op, const char* name, bool may_be_3
   TORCH_CHECK(aligned, op, ": rows of ", name, " must be contiguous and start on 16-byte boundaries");
 }
 
+// Sizes above 1 with their strides, the largest stride first.
+std::vector<std::pair<int64_t, int64_t>> lattice(const Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> d;  // stride, size
+  for (int64_t i = 0; i < t.dim(); i++)
+    if (t.size(i) != 1) d.emplace_back(t.stride(i), t.size(i));
+  std::sort(d.begin(), d.end(), std::greater<>());
+  return d;
+}
+
+// Whether two elements of a tensor may share memory: every stride has to step over all that the smaller
+// strides reach. (torch's own check gives up on tensors with gaps between their rows.)
+bool overlaps_itself(const Tensor& t) {
+  if (t.numel() == 0) return false;
+  const auto d = lattice(t);
+  int64_t reach = 1;
+  for (size_t i = d.size(); i-- > 0;) {
+    if (d[i].first < reach) return true;
+    reach += (d[i].second - 1) * d[i].first;
+  }
+  return false;
+}
+
+void check_no_self_overlap(const Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(!overlaps_itself(t), op, ": ", name, " must not overlap itself");
+}
+
 void check_lengths(const c10::optional<Tensor>& t, int64_t B, const char* op, const char* name) {
   if (!t || !t->defined()) return;
   TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B && t->is_contiguous(), op, ": ", name,
@@ -487,7 +517,7 @@ Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tenso
   };
   weights(gate_up, "w_gate_up", 2 * F, D, p.w_gate_up);
   weights(down, "w_down", D, F, p.w_down);
-  TORCH_CHECK(at::has_internal_overlap(out) != at::MemOverlap::Yes, op, ": out must not overlap itself");
+  check_no_self_overlap(out, op, "out");
   at::assert_no_partial_overlap(out, x);
   if (res) at::assert_no_partial_overlap(out, *residual);
   check_same_cuda(x, {&router, &out}, op);

@@ -89,3 +89,14 @@ def test_stream_partition_model():
             assert c1 - c0 + 1 <= splits(D_, F_, topk, sms)
             for c in range(c0, c1 + 1 if c1 > c0 else c0):  # a tile that several share is each one's first or last
                 assert begin(c) // kc == it or (begin(c + 1) - 1) // kc == it
+
+
+@pytest.mark.skipif(not native.available(), reason="native extension not built")
+@pytest.mark.parametrize("out", [
+    torch.zeros(T * D, dtype=torch.bfloat16).as_strided((T, D), (8, 1)),
+    torch.zeros(T * D, dtype=torch.bfloat16).as_strided((T, D), (0, 1)),
+    torch.zeros(T * D, dtype=torch.bfloat16).as_strided((T, D), (D - 8, 1)),
+])
+def test_refuses_outputs_whose_rows_overlap(out):
+    with pytest.raises(RuntimeError, match="overlap itself"):
+        ops.moe_decode(**dict(args(), out=out))
