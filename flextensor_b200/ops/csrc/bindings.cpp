@@ -357,6 +357,34 @@ void check_no_self_overlap(const Tensor& t, const char* op, const char* name) {
   TORCH_CHECK(!overlaps_itself(t), op, ": ", name, " must not overlap itself");
 }
 
+// Whether some sum of k * stride with |k| < size is d, for strides of a tensor that does not overlap itself:
+// from the largest stride on, at most two k leave a rest that the smaller strides reach.
+bool reaches(const std::vector<std::pair<int64_t, int64_t>>& d, size_t i, int64_t rest) {
+  if (i == d.size()) return rest == 0;
+  const int64_t stride = d[i].first;
+  int64_t below = 0;
+  for (size_t j = i + 1; j < d.size(); j++) below += (d[j].second - 1) * d[j].first;
+  for (int64_t k = (rest - below) / stride - 1; k * stride <= rest + below; k++)
+    if (std::abs(k) < d[i].second && std::abs(rest - k * stride) <= below && reaches(d, i + 1, rest - k * stride)) return true;
+  return false;
+}
+
+// Whether two tensors of one shape and type, of which `a` does not overlap itself, share an element. Views of
+// one buffer with the same strides are told apart exactly (columns side by side share nothing); with
+// different strides, memory ranges that meet count as shared.
+bool shares_memory(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0) return false;
+  const auto da = lattice(a), db = lattice(b);
+  int64_t end_a = 1, end_b = 1;
+  for (const auto& d : da) end_a += (d.second - 1) * d.first;
+  for (const auto& d : db) end_b += (d.second - 1) * d.first;
+  const int64_t bytes = a.element_size();
+  const int64_t gap = static_cast<const char*>(b.const_data_ptr()) - static_cast<const char*>(a.const_data_ptr());
+  if (gap >= end_a * bytes || -gap >= end_b * bytes) return false;
+  if (da != db || gap % bytes) return true;
+  return reaches(da, 0, gap / bytes);
+}
+
 void check_lengths(const c10::optional<Tensor>& t, int64_t B, const char* op, const char* name) {
   if (!t || !t->defined()) return;
   TORCH_CHECK(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B && t->is_contiguous(), op, ": ", name,
@@ -519,7 +547,9 @@ Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tenso
   weights(down, "w_down", D, F, p.w_down);
   check_no_self_overlap(out, op, "out");
   at::assert_no_partial_overlap(out, x);
-  if (res) at::assert_no_partial_overlap(out, *residual);
+  if (res && shares_memory(out, *residual))  // a row of the residual is read by the thread that writes that row of out
+    TORCH_CHECK(residual->const_data_ptr() == out.const_data_ptr() && lattice(*residual) == lattice(out), op,
+                ": out may be residual, but must not overlap it otherwise");
   check_same_cuda(x, {&router, &out}, op);
   if (res) check_same_cuda(x, {&*residual}, op);
   for (int64_t e = 0; e < E; e++) check_same_cuda(x, {&gate_up[e], &down[e]}, op);

@@ -100,3 +100,49 @@ def test_stream_partition_model():
 def test_refuses_outputs_whose_rows_overlap(out):
     with pytest.raises(RuntimeError, match="overlap itself"):
         ops.moe_decode(**dict(args(), out=out))
+
+
+@pytest.mark.skipif(not native.available(), reason="native extension not built")
+@pytest.mark.parametrize("out,residual,refused", [
+    ((0, 2 * D), (2 * D, 2 * D), True),     # one row later in a wide buffer
+    ((0, 2 * D), (8, 2 * D), True),         # columns that overlap
+    ((0, 2 * D), (3 * D, 2 * D), False),    # the other half of the columns, one row later
+    ((0, 2 * D), (D, 2 * D), False),        # the other half of the columns
+    ((0, 2 * D), (0, 2 * D), False),        # the same
+    ((0, 2 * D), (6 * D, 2 * D), False),    # the rows behind
+    ((0, 2 * D), (0, D), True),             # the same memory with other strides
+    ((0, D), (0, 0), True),                 # one row of it for all
+    ((0, D), (2 * D, D), True), ((D, D), (0, D), True), ((0, D), (3 * D, D), False),
+])
+def test_outputs_and_residuals_of_one_buffer(out, residual, refused):
+    buf = bf(20 * D)
+    view = lambda at, stride: buf[at:].as_strided((T, D), (stride, 1), buf.storage_offset() + at)  # noqa: E731
+    with pytest.raises(RuntimeError, match="overlap it otherwise" if refused else "CUDA device"):
+        ops.moe_decode(**dict(args(), out=view(*out), residual=view(*residual)))
+
+
+def test_overlap_model():
+    """The rule of the binding's check against a count of shared elements, for random views of one buffer."""
+    rng = random.Random(1)
+
+    def reaches(d, rest):
+        if not d:
+            return rest == 0
+        (stride, size), low = d[0], d[1:]
+        below = sum((n - 1) * s for s, n in low)
+        quotient = int((rest - below) / stride)  # towards zero, as in C++
+        return any(abs(k) < size and abs(rest - k * stride) <= below and reaches(low, rest - k * stride)
+                   for k in range(quotient - 1, (rest + below) // stride + 1))
+
+    for _ in range(2000):
+        dims, reach = [], 1
+        for _ in range(rng.randint(1, 4)):
+            n, s = rng.randint(2, 5), reach + rng.choice([0, 0, 1, 3, reach])
+            dims.append((s, n))
+            reach += (n - 1) * s
+        dims.sort(reverse=True)
+        offsets = {0}
+        for s, n in dims:
+            offsets = {o + k * s for o in offsets for k in range(n)}
+        d = rng.randint(-reach, reach)
+        assert reaches(dims, d) == bool(offsets & {o + d for o in offsets}), (dims, d)
