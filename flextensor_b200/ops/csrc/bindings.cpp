@@ -413,10 +413,8 @@ void kv_append_q8(const Tensor& k, const Tensor& v, Tensor& kc, Tensor& vc, Tens
   if (!each)
     TORCH_CHECK(pos_all >= 0 && (n_new && n_new->defined() ? pos_all <= L : pos_all + S <= L), op, ": tokens [", pos_all,
                 ", ", pos_all + S, ") do not fit a cache of ", L);
-  for (const Tensor* t : {&kc, &vc, &ks, &vs})
-    TORCH_CHECK(at::has_internal_overlap(*t) != at::MemOverlap::Yes, op, ": the cache must not overlap itself");
-  at::assert_no_overlap(kc, vc);
-  at::assert_no_overlap(ks, vs);
+  for (const Tensor* t : {&kc, &vc, &ks, &vs}) check_no_self_overlap(*t, op, "the cache");
+  TORCH_CHECK(!shares_memory(kc, vc) && !shares_memory(ks, vs), op, ": k and v caches must not overlap");
   check_same_cuda(kc, {&vc, &ks, &vs, &k, &v}, op);
   if (each) check_same_cuda(kc, {&*pos}, op);
   if (n_new && n_new->defined()) check_same_cuda(kc, {&*n_new}, op);

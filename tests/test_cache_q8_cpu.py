@@ -109,3 +109,47 @@ def test_append_refuses_a_cache_that_overlaps_itself():
 def test_attention_refusals(q, kv_len, kw, match):
     with pytest.raises(RuntimeError, match=match):
         ops.decode_attention_q8(q, *cache(), kv_len, block=BLOCK, **kw)
+
+
+def codes(at, strides, l=L):
+    buf = torch.zeros(4 * B * L * HK * 128, dtype=torch.int8)
+    return buf[at:].as_strided((B, l, HK, 128), (*strides, 1), buf.storage_offset() + at), buf
+
+
+@pytest.mark.parametrize("strides,refused", [
+    ((L * HK * 128, HK * 128, 64), True),       # heads half on one another
+    ((L * HK * 128, 128, 128), True),           # a token's second head is the next one's first
+    ((128, 2 * HK * 128, 128), True),           # sequences
+    ((L * HK * 128, 128, L * 128), False),      # heads first
+    ((HK * 128, B * HK * 128, 128), False),     # tokens first
+    ((L * HK * 256, HK * 256, 256), False),     # rows with gaps
+])
+def test_append_refuses_strided_caches_that_overlap_themselves(strides, refused):
+    c = cache()
+    c[0], _ = codes(0, strides)
+    with pytest.raises(RuntimeError, match="overlap itself" if refused else "CUDA device"):
+        ops.kv_append_q8(new(), new(), *c, 0, block=BLOCK)
+    c = cache()
+    c[2] = torch.zeros(64).as_strided((B, 4, HK), (8, 1, 2) if refused else (8, 2, 1))
+    with pytest.raises(RuntimeError, match="overlap itself" if refused else "CUDA device"):
+        ops.kv_append_q8(new(), new(), *c, 0, block=BLOCK)
+
+
+@pytest.mark.parametrize("gap,refused", [(HK * 128, False), (128, True), (0, True), (2 * HK * 128, True), (B * L * 2 * HK * 128, False),
+                                         (L * 2 * HK * 128 + 128, True), (3 * HK * 128, False)])
+def test_append_refuses_strided_caches_that_overlap_one_another(gap, refused):
+    """Keys and values as views of one buffer, [B, L, 2, Hk, 128] where they are side by side."""
+    strides = (L * 2 * HK * 128, 2 * HK * 128, 128)
+    c = cache()
+    c[0], buf = codes(0, strides)
+    c[1] = buf.as_strided((B, L, HK, 128), (*strides, 1), gap)
+    with pytest.raises(RuntimeError, match="must not overlap" if refused else "CUDA device"):
+        ops.kv_append_q8(new(), new(), *c, 0, block=BLOCK)
+    c = cache()
+    both = torch.zeros(B, 4, 2, HK)
+    c[2], c[3] = both[:, :, 0], both[:, :, 1]
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        ops.kv_append_q8(new(), new(), *c, 0, block=BLOCK)
+    c[3] = both[:, :, 0]
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        ops.kv_append_q8(new(), new(), *c, 0, block=BLOCK)
