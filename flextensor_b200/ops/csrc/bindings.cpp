@@ -458,7 +458,7 @@ Tensor decode_attention_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, 
   TORCH_CHECK(Hk > 0 && Hq % Hk == 0, op, ": query heads must be a multiple of kv heads, got ", Hq, " and ", Hk);
   check_lengths(kv_len, B, op, "kv_len");
   TORCH_CHECK(max_len >= 0 && max_len <= L && len_all >= 0 && len_all <= L, op, ": lengths must lie in [0, ", L, "]");
-  TORCH_CHECK(at::has_internal_overlap(o) != at::MemOverlap::Yes, op, ": out must not overlap itself");
+  check_no_self_overlap(o, op, "out");
   check_same_cuda(kc, {&vc, &ks, &vs, &q, &o}, op);
   const bool each = kv_len && kv_len->defined();
   if (each) check_same_cuda(kc, {&*kv_len}, op);

@@ -153,3 +153,14 @@ def test_append_refuses_strided_caches_that_overlap_one_another(gap, refused):
     c[3] = both[:, :, 0]
     with pytest.raises(RuntimeError, match="must not overlap"):
         ops.kv_append_q8(new(), new(), *c, 0, block=BLOCK)
+
+
+@pytest.mark.parametrize("shape,strides,refused", [
+    ((B, 4, 128), (4 * 128, 120, 1), True), ((B, 4, 128), (128, 128, 1), True), ((B, 4, 128), (128, 256, 1), False),
+    ((B, 3, 4, 128), (1536, 128, 128, 1), True), ((B, 3, 4, 128), (1536, 128, 384, 1), False),
+])
+def test_attention_refuses_strided_outputs_that_overlap_themselves(shape, strides, refused):
+    q = torch.zeros(shape, dtype=torch.bfloat16)
+    out = torch.zeros(8192, dtype=torch.bfloat16).as_strided(shape, strides)
+    with pytest.raises(RuntimeError, match="overlap itself" if refused else "CUDA device"):
+        ops.decode_attention_q8(q, *cache(), L, block=BLOCK, out=out)
