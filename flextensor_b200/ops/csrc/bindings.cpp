@@ -411,8 +411,8 @@ void kv_append_q8(const Tensor& k, const Tensor& v, Tensor& kc, Tensor& vc, Tens
   const bool each = pos && pos->defined();
   TORCH_CHECK(S <= L, op, ": ", S, " new tokens do not fit a cache of ", L);
   if (!each)
-    TORCH_CHECK(pos_all >= 0 && (n_new && n_new->defined() ? pos_all <= L : pos_all + S <= L), op, ": tokens [", pos_all,
-                ", ", pos_all + S, ") do not fit a cache of ", L);
+    TORCH_CHECK(pos_all >= 0 && pos_all <= (n_new && n_new->defined() ? L : L - S), op, ": ", S, " tokens from ",
+                pos_all, " on do not fit a cache of ", L);
   for (const Tensor* t : {&kc, &vc, &ks, &vs}) check_no_self_overlap(*t, op, "the cache");
   TORCH_CHECK(!shares_memory(kc, vc) && !shares_memory(ks, vs), op, ": k and v caches must not overlap");
   check_same_cuda(kc, {&vc, &ks, &vs, &k, &v}, op);

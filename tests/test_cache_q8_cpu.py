@@ -164,3 +164,9 @@ def test_attention_refuses_strided_outputs_that_overlap_themselves(shape, stride
     out = torch.zeros(8192, dtype=torch.bfloat16).as_strided(shape, strides)
     with pytest.raises(RuntimeError, match="overlap itself" if refused else "CUDA device"):
         ops.decode_attention_q8(q, *cache(), L, block=BLOCK, out=out)
+
+
+@pytest.mark.parametrize("pos", [2 ** 63 - 1, 2 ** 63 - S, 2 ** 31, -2 ** 63])
+def test_append_refuses_positions_past_any_cache(pos):
+    with pytest.raises(RuntimeError, match="do not fit"):
+        ops.kv_append_q8(new(), new(), *cache(), pos, block=BLOCK)
