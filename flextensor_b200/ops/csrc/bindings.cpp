@@ -284,6 +284,9 @@ void decode_attention(const Tensor& q, const Tensor& kc, const Tensor& vc, Tenso
 // refused call says why on any machine.
 constexpr int64_t kHead = 128;
 
+// strides of a dimension that 16-byte accesses can take; a single entry may have any
+bool stride_of(const Tensor& t, int64_t dim, int64_t multiple) { return t.size(dim) == 1 || t.stride(dim) % multiple == 0; }
+
 bool on_16_bytes(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0; }
 
 void check_cache(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs, int64_t block, const char* op) {
@@ -301,8 +304,7 @@ void check_cache(const Tensor& kc, const Tensor& vc, const Tensor& ks, const Ten
               op, ": scales must be fp32 [B, ceil(L / block), Hk] = ", want, ", got ", ks.sizes(), " and ",
               vs.sizes());
   for (const Tensor* t : {&kc, &vc}) {
-    TORCH_CHECK(t->stride(3) == 1 && t->stride(0) % 16 == 0 && t->stride(1) % 16 == 0 && t->stride(2) % 16 == 0 &&
-                    on_16_bytes(*t),
+    TORCH_CHECK(t->stride(3) == 1 && stride_of(*t, 0, 16) && stride_of(*t, 1, 16) && stride_of(*t, 2, 16) && on_16_bytes(*t),
                 op, ": cache rows must be contiguous and start on 16-byte boundaries");
   }
 }
@@ -327,7 +329,7 @@ void check_rows(const Tensor& t, const char* op, const char* name, bool may_be_3
   TORCH_CHECK((d == 4 || (d == 3 && may_be_3d)) && t.size(d - 1) == kHead, op, ": ", name, " must be [B, S, H, 128]",
               may_be_3d ? " or [B, H, 128]" : "", ", got ", t.sizes());
   bool aligned = t.stride(d - 1) == 1 && on_16_bytes(t);
-  for (int64_t i = 0; i + 1 < d; i++) aligned = aligned && t.stride(i) % 8 == 0;
+  for (int64_t i = 0; i + 1 < d; i++) aligned = aligned && stride_of(t, i, 8);
   TORCH_CHECK(aligned, op, ": rows of ", name, " must be contiguous and start on 16-byte boundaries");
 }
 
@@ -501,7 +503,7 @@ Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tenso
     TORCH_CHECK(t.scalar_type() == at::kBFloat16, op, ": ", name, " must be bfloat16");
     TORCH_CHECK(t.dim() == 2 && t.size(0) == r && t.size(1) == c, op, ": ", name, " must be [", r, ", ", c, "], got ",
                 t.sizes());
-    TORCH_CHECK(t.stride(1) == 1 && t.stride(0) % 8 == 0 && on_16_bytes(t), op, ": rows of ", name,
+    TORCH_CHECK(t.stride(1) == 1 && stride_of(t, 0, 8) && on_16_bytes(t), op, ": rows of ", name,
                 " must be contiguous and start on 16-byte boundaries");
   };
   TORCH_CHECK(x.dim() == 2 && router.dim() == 2, op, ": x must be [T, D] and router [E, D], got ", x.sizes(), " and ",

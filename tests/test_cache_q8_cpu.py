@@ -170,3 +170,16 @@ def test_attention_refuses_strided_outputs_that_overlap_themselves(shape, stride
 def test_append_refuses_positions_past_any_cache(pos):
     with pytest.raises(RuntimeError, match="do not fit"):
         ops.kv_append_q8(new(), new(), *cache(), pos, block=BLOCK)
+
+
+def test_single_entries_may_have_any_stride():
+    """A dimension of one entry is never stepped over: its stride does not matter (contiguous() leaves it
+    as it is, so a caller could not mend it)."""
+    odd = lambda t: t.as_strided(t.shape, [3 if n == 1 else s for n, s in zip(t.shape, t.stride())])  # noqa: E731
+    c = [odd(t) if t.dim() == 4 else t for t in cache(b=1, l=1, hk=1)]
+    x = odd(new(b=1, s=1, hk=1))
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        ops.kv_append_q8(x, x, *c, 0, block=BLOCK)
+    for q in (odd(torch.zeros(1, 1, 128, dtype=torch.bfloat16)), x):
+        with pytest.raises(RuntimeError, match="CUDA device"):
+            ops.decode_attention_q8(q, *c, 1, block=BLOCK, out=odd(torch.zeros_like(q)))

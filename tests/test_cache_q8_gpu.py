@@ -472,3 +472,15 @@ def test_attention_infinite_value_scales_stay():
     n = torch.tensor([49], dtype=torch.int32, device=DEV)  # query 0 sees 48 keys, none of block 3
     got = ops.decode_attention_q8(q, *cache, n, block=block)
     assert torch.equal(got[:, :1], ops.decode_attention_q8(q, *clean, n, block=block)[:, :1]) and not got[:, 1:].isfinite().any()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_single_entries_may_have_any_stride(fmt):
+    """One sequence, head, token: strides of those dimensions that no access could take."""
+    odd = lambda t: t.as_strided(t.shape, [3 if n == 1 else s for n, s in zip(t.shape, t.stride())])  # noqa: E731
+    for B, L, Hk, S in ((1, 1, 1, 1), (1, 100, 2, 1), (2, 70, 1, 3)):
+        cache = [odd(c) for c in junk_cache(fmt, B, L, Hk, 32, 45)]
+        k, v = odd(bf16(46, B, S, Hk, 128)), odd(bf16(47, B, S, Hk, 128))
+        check_append(k, v, cache, [L - S] * B, [S] * B, 32, fmt, pos_arg=L - S)
+        q = odd(bf16(48, B, S, 2 * Hk, 128, spread=False))
+        check_attend(q, cache, [L] * B, 32, L, out=odd(torch.zeros(q.shape, device=DEV, dtype=torch.bfloat16)))

@@ -146,3 +146,13 @@ def test_overlap_model():
             offsets = {o + k * s for o in offsets for k in range(n)}
         d = rng.randint(-reach, reach)
         assert reaches(dims, d) == bool(offsets & {o + d for o in offsets}), (dims, d)
+
+
+@pytest.mark.skipif(not native.available(), reason="native extension not built")
+@pytest.mark.parametrize("stride", [0, 1, 3])
+def test_a_single_row_may_have_any_stride(stride):
+    row = lambda: bf(1, D).as_strided((1, D), (stride, 1))  # noqa: E731
+    a = dict(args(t=1, e=1), topk=1)
+    a.update(x=row(), router=row(), residual=row(), out=row())
+    with pytest.raises(RuntimeError, match="CUDA device"):
+        ops.moe_decode(**a)

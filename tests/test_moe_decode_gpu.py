@@ -149,3 +149,21 @@ def test_streams_and_graphs():
         assert all(torch.equal(a, want) for a in again)
         assert torch.equal(got, ops.moe_decode(**dict(p, x=fresh), topk=2, residual=res))
     assert native.device_error(reset=True) == 0
+
+
+def test_single_row_of_any_stride():
+    p, res = make(1, 256, 192, 1, seed=8)
+    odd = lambda t: t.as_strided(t.shape, (3, 1))  # noqa: E731
+    want = check(p, 1, residual=res)
+    got = ops.moe_decode(**dict(p, x=odd(p["x"]), router=odd(p["router"])), topk=1, residual=odd(res), out=odd(torch.zeros_like(res)))
+    assert torch.equal(got, want)
+
+
+def test_halves_of_a_wide_buffer():
+    """The output beside the residual in one buffer: columns side by side share no memory."""
+    p, res = make(9, 256, 192, 4, seed=9)
+    want = check(p, 2, residual=res)
+    wide = torch.zeros(9, 512, device=DEV, dtype=torch.bfloat16)
+    wide[:, 256:] = res
+    assert torch.equal(ops.moe_decode(**p, topk=2, residual=wide[:, 256:], out=wide[:, :256]), want)
+    assert torch.equal(wide[:, 256:], res)
