@@ -1052,6 +1052,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("max_len"), py::arg("block"), py::arg("scale"));
   m.def("moe_decode", &moe_decode, py::arg("x"), py::arg("router"), py::arg("w_gate_up"), py::arg("w_down"),
         py::arg("topk"), py::arg("residual"), py::arg("out"));
+  m.def("moe_decode_one_map", [](const std::vector<uint64_t>& w) {
+    std::vector<const __nv_bfloat16*> p;
+    for (uint64_t a : w) p.push_back(reinterpret_cast<const __nv_bfloat16*>(a));
+    return ft::moe_decode_one_map(p.data(), (int)p.size());
+  });
   m.def("p2p_publish_raw", &p2p_publish_raw);
   m.def("tp_ag_gemm", &tp_ag_gemm, py::arg("a_full"), py::arg("w"), py::arg("out"), py::arg("bias"), py::arg("epi"),
         py::arg("peer_a"), py::arg("flags"), py::arg("flag_stride"), py::arg("peer_acks"), py::arg("rank"),

@@ -27,6 +27,9 @@ struct MoeDecodeProblem {
   void* workspace = nullptr;              // moe_decode_workspace(p) bytes, 256-byte aligned
 };
 size_t moe_decode_workspace(const MoeDecodeProblem& p);
+// Whether one tensor map serves all experts: their weights lie at equal distances that a map can hold (a
+// multiple of 16 bytes below 2^40). Else each has a map of its own.
+bool moe_decode_one_map(const __nv_bfloat16* const* w, int E);
 // four kernels
 cudaError_t moe_decode(const MoeDecodeProblem& p, cudaStream_t stream);
 int moe_decode_device_error(bool reset);

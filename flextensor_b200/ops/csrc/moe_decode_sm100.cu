@@ -722,16 +722,6 @@ bool weight_maps(Maps<N>& m, const __nv_bfloat16* const* w, int E, int inner, in
   }
 }
 
-// one tensor map serves all experts when their weights lie at equal distances
-bool evenly_spaced(const __nv_bfloat16* const* w, int E) {
-  if (E == 1) return true;
-  const long long d = w[1] - w[0];
-  if (d <= 0 || d % 8) return false;
-  for (int e = 2; e < E; e++)
-    if (w[e] - w[e - 1] != d) return false;
-  return true;
-}
-
 template <class... P, class... A>
 cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, const A&... args) {
   cudaLaunchConfig_t cfg = {};
@@ -778,13 +768,22 @@ cudaError_t launch_product(const MoeDecodeProblem& p, Args a, cudaStream_t strea
 
 template <bool UP>
 cudaError_t launch_product_for(const MoeDecodeProblem& p, const Args& a, cudaStream_t stream) {
-  if (evenly_spaced(UP ? p.w_gate_up : p.w_down, p.E)) return launch_product<UP, 1>(p, a, stream);
+  if (moe_decode_one_map(UP ? p.w_gate_up : p.w_down, p.E)) return launch_product<UP, 1>(p, a, stream);
   if (p.E <= 8) return launch_product<UP, 8>(p, a, stream);
   if (p.E <= 32) return launch_product<UP, 32>(p, a, stream);
   return launch_product<UP, MAX_E>(p, a, stream);
 }
 
 }  // namespace
+
+bool moe_decode_one_map(const __nv_bfloat16* const* w, int E) {
+  if (E == 1) return true;
+  const long long d = reinterpret_cast<intptr_t>(w[1]) - reinterpret_cast<intptr_t>(w[0]);  // bytes
+  if (d <= 0 || d % 16 || d >= (1LL << 40)) return false;
+  for (int e = 2; e < E; e++)
+    if (reinterpret_cast<intptr_t>(w[e]) - reinterpret_cast<intptr_t>(w[e - 1]) != d) return false;
+  return true;
+}
 
 size_t moe_decode_workspace(const MoeDecodeProblem& p) { return layout_of(p).bytes; }
 

@@ -156,3 +156,16 @@ def test_a_single_row_may_have_any_stride(stride):
     a.update(x=row(), router=row(), residual=row(), out=row())
     with pytest.raises(RuntimeError, match="CUDA device"):
         ops.moe_decode(**a)
+
+
+@pytest.mark.skipif(not native.available(), reason="native extension not built")
+@pytest.mark.parametrize("distances,one", [
+    ([], True), ([1 << 20] * 7, True), ([16] * 3, True), ([(1 << 40) - 16], True),
+    ([1 << 40], False), ([1 << 41] * 3, False),           # farther than a tensor map's stride reaches
+    ([1 << 20, 1 << 20, 1 << 21], False), ([-(1 << 20)] * 3, False), ([0, 0], False), ([8], False),
+])
+def test_one_tensor_map_for_all_experts(distances, one):
+    w = [1 << 44]
+    for d in distances:
+        w.append(w[-1] + d)
+    assert native.lib().moe_decode_one_map(w) == one
