@@ -42,7 +42,8 @@ class MixtralConfig(LlamaConfig):
     rope_theta: float = 1000000.0
     n_experts: int = 8
     topk: int = 2
-    moe_decode: bool = False  # single GPU, native path: steps of at most 64 tokens take ops.moe_decode
+    # single GPU, native path: steps of at most 64 tokens take ops.moe_decode (with at most 128 experts, 8 a token)
+    moe_decode: bool = False
 
 
 MIXTRAL_8X22B = MixtralConfig()
@@ -106,7 +107,7 @@ class MixtralLayer(nn.Module):
             x = self.attn.attention_torch(x, B, S, rope)
         h = ops.rmsnorm(x, self.ffn_norm, eps=cfg.eps) if impl == "fused" else _rms_torch(x, self.ffn_norm, cfg.eps)
         if (ep is None and impl == "fused" and cfg.moe_decode and h.shape[0] <= ops.MOE_DECODE_MAX_TOKENS
-                and len(self.experts) == cfg.n_experts):
+                and len(self.experts) == cfg.n_experts <= ops.MOE_DECODE_MAX_EXPERTS and cfg.topk <= ops.MOE_DECODE_MAX_TOPK):
             return ops.moe_decode(h, self.router, [e.w_gate_up for e in self.experts],
                                   [e.w_down for e in self.experts], cfg.topk, residual=x, out=x)
         ids, wts = route_topk(h, self.router, cfg.topk)

@@ -13,7 +13,9 @@ from flextensor_b200.ops.api import (
     layernorm_modulate,
     linear,
     linear_swiglu,
+    MOE_DECODE_MAX_EXPERTS,
     MOE_DECODE_MAX_TOKENS,
+    MOE_DECODE_MAX_TOPK,
     moe_decode,
     qk_rmsnorm_rope,
     rmsnorm,
@@ -26,5 +28,5 @@ from flextensor_b200.ops.api import (
 )
 
 __all__ = ["EPI", "TP_EPI", "attention", "attention_cp", "decode_attention", "decode_attention_q8", "kv_append_q8", "launch_count", "layernorm_modulate", "linear",
-           "linear_swiglu", "MOE_DECODE_MAX_TOKENS", "moe_decode", "qk_rmsnorm_rope", "rmsnorm", "rope", "tp_ag_counter_words", "tp_allgather_gemm", "tp_gemm_reducescatter",
+           "linear_swiglu", "MOE_DECODE_MAX_EXPERTS", "MOE_DECODE_MAX_TOKENS", "MOE_DECODE_MAX_TOPK", "moe_decode", "qk_rmsnorm_rope", "rmsnorm", "rope", "tp_ag_counter_words", "tp_allgather_gemm", "tp_gemm_reducescatter",
            "tp_reduce", "tp_rmsnorm"]

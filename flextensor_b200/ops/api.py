@@ -194,6 +194,8 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
 
 
 MOE_DECODE_MAX_TOKENS = 64
+MOE_DECODE_MAX_EXPERTS = 128
+MOE_DECODE_MAX_TOPK = 8
 
 
 def moe_decode(x: torch.Tensor, router: torch.Tensor, w_gate_up, w_down, topk: int, *,
