@@ -72,6 +72,14 @@ class MixtralLayer(nn.Module):
         self.expert_ids = list(range(cfg.n_experts)) if expert_ids is None else list(expert_ids)
         self.experts = nn.ModuleList([Expert(cfg.dim, cfg.ffn_dim) for _ in self.expert_ids])
 
+    def all_experts(self):
+        """The experts in the order of the router's rows; None if some are not here."""
+        ids = list(range(self.cfg.n_experts))
+        if self.expert_ids == ids:
+            return self.experts
+        at = dict(zip(self.expert_ids, self.experts))
+        return [at[e] for e in ids] if sorted(self.expert_ids) == ids else None
+
     def moe_single(self, h: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, out: torch.Tensor, impl: str):
         from flextensor_b200 import ops
 
@@ -106,10 +114,11 @@ class MixtralLayer(nn.Module):
         else:
             x = self.attn.attention_torch(x, B, S, rope)
         h = ops.rmsnorm(x, self.ffn_norm, eps=cfg.eps) if impl == "fused" else _rms_torch(x, self.ffn_norm, cfg.eps)
-        if (ep is None and impl == "fused" and cfg.moe_decode and h.shape[0] <= ops.MOE_DECODE_MAX_TOKENS
-                and len(self.experts) == cfg.n_experts <= ops.MOE_DECODE_MAX_EXPERTS and cfg.topk <= ops.MOE_DECODE_MAX_TOPK):
-            return ops.moe_decode(h, self.router, [e.w_gate_up for e in self.experts],
-                                  [e.w_down for e in self.experts], cfg.topk, residual=x, out=x)
+        if ep is None and impl == "fused" and cfg.moe_decode and h.shape[0] <= ops.MOE_DECODE_MAX_TOKENS:
+            experts = self.all_experts()
+            if experts is not None and cfg.n_experts <= ops.MOE_DECODE_MAX_EXPERTS and cfg.topk <= ops.MOE_DECODE_MAX_TOPK:
+                return ops.moe_decode(h, self.router, [e.w_gate_up for e in experts], [e.w_down for e in experts],
+                                      cfg.topk, residual=x, out=x)
         ids, wts = route_topk(h, self.router, cfg.topk)
         if ep is None:
             return self.moe_single(h, ids, wts, x, impl)

@@ -159,3 +159,26 @@ def test_streamed_decode_is_bitwise():
                 assert torch.equal(a, b)
     assert om.phase.value == "inference"
     assert native.device_error(reset=True) == 0
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("kw,ids", [(dict(n_experts=4), [2, 0, 3, 1]), (dict(n_experts=130, ffn_dim=64), None),
+                                    (dict(n_experts=12, topk=10), None)])
+def test_layers_with_and_without_the_few_token_path(kw, ids):
+    """Experts kept in another order than their ids; more experts, or more a token, than the one call takes."""
+    from flextensor_b200.models.llama import rope_tables_1d
+    from flextensor_b200.models.mixtral import MixtralLayer
+
+    cfg = tiny_mixtral(dim=256, n_heads=2, n_kv_heads=1, moe_decode=True, **kw)
+    m = MixtralLayer(cfg, ids).to(DEV)
+    g = torch.Generator(device=DEV).manual_seed(8)
+    for p in m.parameters():
+        p.normal_(0.0, 0.06, generator=g)
+    m = m.to(torch.bfloat16)
+    x = torch.randn(9, cfg.dim, device=DEV, generator=g).bfloat16()
+    rope = rope_tables_1d(9, cfg.head_dim, cfg.rope_theta, DEV)
+    a = m(x.clone(), 1, 9, rope)
+    cfg.moe_decode = False
+    b = m(x.clone(), 1, 9, rope)
+    assert near(a, b, 2 ** -7)  # one rounding of each path's output, and of the loop's h
+    assert native.device_error(reset=True) == 0

@@ -41,3 +41,15 @@ def test_path(step, tokens, kw, path):
     assert step(m, tokens)[0] == path
     m.cfg.moe_decode = False
     assert step(m, tokens)[0] == "loop"
+
+
+def test_experts_go_by_their_ids(step):
+    """The router's row e belongs to the expert whose id is e, wherever the layer keeps it."""
+    m = layer(expert_ids=[2, 0, 3, 1])
+    path, weights = step(m, 3)
+    assert path == "decode"
+    for e, (gate_up, down) in enumerate(weights):
+        mine = m.experts[m.expert_ids.index(e)]
+        assert gate_up is mine.w_gate_up and down is mine.w_down
+    assert step(layer(expert_ids=[0, 1]), 3)[0] == "loop"
+    assert step(layer(expert_ids=[0, 1, 1, 2]), 3)[0] == "loop"
