@@ -176,20 +176,16 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     a sequence's others should lie within 2**90 of one another).
 
     ``q [B, Hq, 128]``, or ``[B, Sq, Hq, 128]`` for the last Sq tokens of each sequence, whose keys
-    are in the cache already (a few: the workspace grows with Sq): query i sees keys ``[0, kv_len - Sq + 1 + i)``; one that sees none
-    gets zeros. ``kv_len``: an int or an int32 CUDA tensor ``[B]`` (then ``max_len``, default L,
+    are in the cache already: query i sees keys ``[0, kv_len - Sq + 1 + i)``; one that sees none gets
+    zeros. Made for a few queries: every 16 rows (queries x heads) of a KV head pass over its cache once. ``kv_len``: an int or an int32 CUDA tensor ``[B]`` (then ``max_len``, default L,
     bounds it: longer ones are cut)."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
-    if isinstance(kv_len, torch.Tensor):
-        ml = k_cache.shape[1] if max_len is None else max_len
-        out = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, kv_len, 0, ml, block, scale)
-    else:
-        ml = kv_len
-        out = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, None, kv_len, kv_len, block,
-                                               scale)
-    if q.numel():
-        _count(2 if ml > 0 else 1)  # the attention, if there are keys, and the merge of its partial results
+    lens, kv_len, max_len = (kv_len, 0, k_cache.shape[1] if max_len is None else max_len) \
+        if isinstance(kv_len, torch.Tensor) else (None, kv_len, kv_len)
+    out, launches = native.lib().decode_attention_q8(q, k_cache, v_cache, k_scale, v_scale, out, lens, kv_len, max_len,
+                                                     block, scale)
+    _count(launches)  # the attention, if there are keys, and the merge of its partial results
     return out
 
 

@@ -443,7 +443,12 @@ void kv_append_q8(const Tensor& k, const Tensor& v, Tensor& kc, Tensor& vc, Tens
   check_ok(ft::cache_append(p, at::cuda::getCurrentCUDAStream()), op);
 }
 
-Tensor decode_attention_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
+// A call's workspace holds partial results of every query row; calls of more queries than fit take them in
+// several launches, which costs nothing: each 16 rows of a KV head pass over the cache by themselves anyway.
+constexpr size_t kCacheDecodeScratchBytes = size_t(256) << 20;
+
+// the output, and the number of kernels launched
+std::pair<Tensor, int> decode_attention_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& ks, const Tensor& vs,
                            const c10::optional<Tensor>& o_given, const c10::optional<Tensor>& kv_len, int64_t len_all,
                            int64_t max_len, int64_t block, double scale) {
   const char* op = "decode_attention_q8";
@@ -473,11 +478,9 @@ Tensor decode_attention_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, 
   p.L = (int)L;
   p.block = (int)block;
   p.format = kc.scalar_type() == at::kChar ? ft::CACHE_INT8 : ft::CACHE_E4M3;
-  p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
   p.q_b = q.stride(0);
   p.q_tok = many ? q.stride(1) : 0;
   p.q_h = q.stride(many ? 2 : 1);
-  p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr());
   p.o_b = o.stride(0);
   p.o_tok = many ? o.stride(1) : 0;
   p.o_h = o.stride(many ? 2 : 1);
@@ -488,11 +491,24 @@ Tensor decode_attention_q8(const Tensor& q, const Tensor& kc, const Tensor& vc, 
   p.max_len = (int)(each ? max_len : len_all);
   p.scale = (float)scale;
   p.num_sms = num_sms_for(kc.get_device());
-  if (q.numel() == 0) return o;
+  if (q.numel() == 0) return {o, 0};
+  while (p.Sq > 1 && ft::cache_decode_scratch_floats(p) * sizeof(float) > kCacheDecodeScratchBytes) p.Sq = (p.Sq + 1) / 2;
+  const int step = p.Sq;
+  if (step < Sq && shares_memory(o, q))  // a launch's outputs are written before the next one's queries are read
+    TORCH_CHECK(q.const_data_ptr() == o.const_data_ptr() && lattice(q) == lattice(o), op,
+                ": out may be q, but must not overlap it otherwise");
   const auto scratch = c10::cuda::CUDACachingAllocator::get()->allocate(ft::cache_decode_scratch_floats(p) * sizeof(float));
   p.scratch = static_cast<float*>(scratch.get());
-  check_ok(ft::cache_decode(p, at::cuda::getCurrentCUDAStream()), op);
-  return o;
+  int launches = 0;
+  for (int64_t first = 0; first < Sq; first += step) {
+    p.Sq = (int)std::min<int64_t>(step, Sq - first);
+    p.later = (int)(Sq - first - p.Sq);
+    p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr()) + first * p.q_tok;
+    p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr()) + first * p.o_tok;
+    check_ok(ft::cache_decode(p, at::cuda::getCurrentCUDAStream()), op);
+    launches += p.max_len > p.later ? 2 : 1;
+  }
+  return {o, launches};
 }
 
 Tensor moe_decode(const Tensor& x, const Tensor& router, const std::vector<Tensor>& gate_up,

@@ -259,7 +259,7 @@ struct DecArgs {
   CacheSide k, v;
   int one_b[2], one_h[2];               // keys / values: the cache is broadcast over sequences / heads (stride 0)
   const int* kv_len;
-  int len_all, max_len;
+  int len_all, max_len, later;          // later: tokens of each sequence behind the last query's
   float scale_log2;                     // softmax scale * log2(e)
   float* part_o;                        // [steps of heads + runs][WARPS][8 * NT][128]
   float2* part_ml;                      // [steps of heads + runs][WARPS][8 * NT] reference and sum
@@ -561,7 +561,7 @@ __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT
 }
 
 __device__ __forceinline__ int seq_len(const DecArgs& a, int b) {
-  return max(0, min(a.kv_len ? a.kv_len[b] : a.len_all, a.max_len));
+  return max(0, min(a.kv_len ? a.kv_len[b] : a.len_all, a.max_len) - a.later);
 }
 __device__ __forceinline__ int seq_units(const DecArgs& a, int b) { return (seq_len(a, b) + UNIT - 1) / UNIT; }
 
@@ -1080,6 +1080,7 @@ cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream) {
   a.kv_len = p.kv_len;
   a.len_all = p.len_all;
   a.max_len = p.max_len;
+  a.later = p.later;
   a.scale_log2 = p.scale * 1.4426950408889634f;
   a.heads = heads_of(p);
   a.keys = WARPS / a.heads;
@@ -1095,7 +1096,7 @@ cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream) {
   const long long expect = (a.runs / head_steps_of(p) + 1) * a.keys;
   a.merge_per_row = expect >= 64 ? 16 : expect >= 32 ? 8 : expect >= 16 ? 4 : expect >= 8 ? 2 : 1;
   const bool one = col_tiles(p) == 1;
-  if (p.max_len > 0) {  // without keys there may be no memory to map; the merge alone writes the zeros
+  if (p.max_len > p.later) {  // without keys there may be no memory to map; the merge alone writes the zeros
     CUtensorMap tk, tv;
     if (!side_map(&tk, p.side[0], p, a.one_b[0], a.one_h[0]) || !side_map(&tv, p.side[1], p, a.one_b[1], a.one_h[1]))
       return cudaErrorInvalidValue;

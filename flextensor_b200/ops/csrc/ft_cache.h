@@ -38,12 +38,13 @@ struct CacheDecodeProblem {
   const int* kv_len = nullptr;             // [B]; null: len_all
   int len_all = 0;
   int max_len = 0;                         // bound of the lengths: a longer one is cut to it
+  int later = 0;                           // tokens of each sequence that follow the Sq queries'
   float scale = 1.f;
   int num_sms = 148;
   float* scratch = nullptr;                // cache_decode_scratch_floats(p) floats
 };
 size_t cache_decode_scratch_floats(const CacheDecodeProblem& p);
-// two kernels; where max_len is 0, the second alone
+// two kernels; where no key may count (max_len <= later), the second alone
 cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream);
 int cache_device_error(bool reset);
 

@@ -484,3 +484,52 @@ def test_single_entries_may_have_any_stride(fmt):
         check_append(k, v, cache, [L - S] * B, [S] * B, 32, fmt, pos_arg=L - S)
         q = odd(bf16(48, B, S, 2 * Hk, 128, spread=False))
         check_attend(q, cache, [L] * B, 32, L, out=odd(torch.zeros(q.shape, device=DEV, dtype=torch.bfloat16)))
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_attention_of_many_queries(ragged):
+    """1000 queries a sequence, as where a prompt is continued: the workspace stays below 256 MB (one launch
+    for all would take 512 MB), and lengths shorter than the queries leave rows without keys."""
+    B, Sq, L, Hq, Hk, block = 16, 1000, 1100, 64, 8, 64
+    cache = junk_cache("int8", B, L, Hk, block, 51)
+    q = bf16(52, B, Sq, Hq, 128, spread=False)
+    lens = [L] * B
+    if ragged:
+        lens = torch.randint(0, L + 1, (B,), generator=torch.Generator().manual_seed(4)).tolist()
+        lens[:4] = [0, 1, 999, 1000]
+    kv_len = torch.tensor(lens, dtype=torch.int32, device=DEV) if ragged else L
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before, launches = torch.cuda.memory_allocated(), ops.launch_count()
+    ops.decode_attention_q8(q, *cache, kv_len, block=block, out=out)
+    assert torch.cuda.max_memory_allocated() - before <= 257 << 20
+    assert ops.launch_count() - launches > 2
+    g = torch.Generator().manual_seed(5)
+    for b in range(B):
+        j = torch.arange(lens[b], device=DEV) // block
+        for i in torch.randint(0, Sq, (4,), generator=g).tolist() + [0, Sq - 1]:
+            m, h = lens[b] - Sq + 1 + i, int(torch.randint(0, Hq, (1,), generator=g))
+            if m <= 0:
+                assert bool((out[b, i] == 0).all())
+                continue
+            k = cache[0][b, :m, h // 8].double() * cache[2][b, j[:m], h // 8].double()[:, None]
+            v = cache[1][b, :m, h // 8].double() * cache[3][b, j[:m], h // 8].double()[:, None]
+            p = torch.softmax(k @ q[b, i, h].double() * 128 ** -0.5, 0)
+            err = (out[b, i, h].double() - p @ v).abs()
+            assert bool((err <= (p @ v).abs() * 2 ** -8 + (p @ v.abs()) * 2 ** -9).all())
+    assert native.device_error(reset=True) == 0
+
+
+def test_attention_of_many_queries_in_place():
+    """Several launches: out may be q itself; another overlap is refused."""
+    B, Sq, L, Hq, Hk, block = 32, 300, 320, 64, 1, 64
+    cache = junk_cache("e4m3", B, L, Hk, block, 53)
+    buf = torch.randn(B * Sq * Hq * 128 + 128, device=DEV, generator=torch.Generator(device=DEV).manual_seed(54)).bfloat16()
+    q, shifted = buf[:-128].view(B, Sq, Hq, 128), buf[128:].view(B, Sq, Hq, 128)
+    launches = ops.launch_count()
+    want = ops.decode_attention_q8(q, *cache, L, block=block)
+    assert ops.launch_count() - launches > 2
+    with pytest.raises(RuntimeError, match="overlap it otherwise"):
+        ops.decode_attention_q8(q, *cache, L, block=block, out=shifted)
+    assert torch.equal(ops.decode_attention_q8(q, *cache, L, block=block, out=q), want)
