@@ -7,6 +7,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/util/SmallVector.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -334,8 +335,9 @@ void check_rows(const Tensor& t, const char* op, const char* name, bool may_be_3
 }
 
 // Sizes above 1 with their strides, the largest stride first.
-std::vector<std::pair<int64_t, int64_t>> lattice(const Tensor& t) {
-  std::vector<std::pair<int64_t, int64_t>> d;  // stride, size
+using Lattice = c10::SmallVector<std::pair<int64_t, int64_t>, 5>;  // stride, size
+Lattice lattice(const Tensor& t) {
+  Lattice d;
   for (int64_t i = 0; i < t.dim(); i++)
     if (t.size(i) != 1) d.emplace_back(t.stride(i), t.size(i));
   std::sort(d.begin(), d.end(), std::greater<>());
@@ -345,7 +347,7 @@ std::vector<std::pair<int64_t, int64_t>> lattice(const Tensor& t) {
 // Whether two elements of a tensor may share memory: every stride has to step over all that the smaller
 // strides reach. (torch's own check gives up on tensors with gaps between their rows.)
 bool overlaps_itself(const Tensor& t) {
-  if (t.numel() == 0) return false;
+  if (t.is_non_overlapping_and_dense() || t.numel() == 0) return false;
   const auto d = lattice(t);
   int64_t reach = 1;
   for (size_t i = d.size(); i-- > 0;) {
@@ -361,7 +363,7 @@ void check_no_self_overlap(const Tensor& t, const char* op, const char* name) {
 
 // Whether some sum of k * stride with |k| < size is d, for strides of a tensor that does not overlap itself:
 // from the largest stride on, at most two k leave a rest that the smaller strides reach.
-bool reaches(const std::vector<std::pair<int64_t, int64_t>>& d, size_t i, int64_t rest) {
+bool reaches(const Lattice& d, size_t i, int64_t rest) {
   if (i == d.size()) return rest == 0;
   const int64_t stride = d[i].first;
   int64_t below = 0;
@@ -376,14 +378,16 @@ bool reaches(const std::vector<std::pair<int64_t, int64_t>>& d, size_t i, int64_
 // different strides, memory ranges that meet count as shared.
 bool shares_memory(const Tensor& a, const Tensor& b) {
   if (a.numel() == 0) return false;
-  const auto da = lattice(a), db = lattice(b);
-  int64_t end_a = 1, end_b = 1;
-  for (const auto& d : da) end_a += (d.second - 1) * d.first;
-  for (const auto& d : db) end_b += (d.second - 1) * d.first;
   const int64_t bytes = a.element_size();
+  auto end = [&](const Tensor& t) {
+    int64_t n = 1;
+    for (int64_t i = 0; i < t.dim(); i++) n += (t.size(i) - 1) * t.stride(i);
+    return n * bytes;
+  };
   const int64_t gap = static_cast<const char*>(b.const_data_ptr()) - static_cast<const char*>(a.const_data_ptr());
-  if (gap >= end_a * bytes || -gap >= end_b * bytes) return false;
-  if (da != db || gap % bytes) return true;
+  if (gap >= end(a) || -gap >= end(b)) return false;
+  const auto da = lattice(a);
+  if (da != lattice(b) || gap % bytes) return true;
   return reaches(da, 0, gap / bytes);
 }
 
