@@ -23,7 +23,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from flextensor_b200.models.kv_cache import QuantizedKV, attend, check_draft, new_layer_cache, store
+from flextensor_b200.models.kv_cache import QuantizedKV, attend, check_draft, new_layer_cache, rewind, store
 
 
 @dataclass
@@ -254,7 +254,9 @@ class LlamaModel(nn.Module):
     def decode_step(self, token: torch.Tensor, cache, pos: int) -> torch.Tensor:
         """One new token per sequence at position ``pos``; returns its logits ``[B, vocab]``. On an 8-bit
         cache ``token`` may be ``[B, S]``, S > 1, the tokens of positions ``[pos, pos + S)`` (a draft to
-        check); the logits are then ``[B, S, vocab]``."""
+        check); the logits are then ``[B, S, vocab]``. Where only the first are accepted, :meth:`rewind`
+        takes the others back before the next step: left there, they would keep the scale of the block
+        they share with the tokens before them."""
         B = token.shape[0]
         S = check_draft(token, cache)
         x = self.embed(token.reshape(B * S)).contiguous()
@@ -264,6 +266,12 @@ class LlamaModel(nn.Module):
             x = layer(x, B, S, rope_p, self.impl, cache=c, pos=pos)
         logits = self._logits(x)
         return logits if S == 1 else logits.view(B, S, -1)
+
+    @torch.no_grad()
+    def rewind(self, cache, pos: int) -> None:
+        """Take back the tokens from position ``pos`` on of the last :meth:`decode_step`, a draft of 2 to 16
+        tokens of which only the first were accepted (:func:`flextensor_b200.models.kv_cache.rewind`)."""
+        rewind(cache, pos)
 
     @torch.no_grad()
     def generate(self, tokens: torch.Tensor, max_new: int, cache_dtype=torch.bfloat16) -> torch.Tensor:

@@ -27,7 +27,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from flextensor_b200.models.kv_cache import check_draft, new_layer_cache
+from flextensor_b200.models.kv_cache import check_draft, new_layer_cache, rewind
 from flextensor_b200.models.llama import LlamaConfig, LlamaLayer, _rms_torch, rope_tables_1d
 
 
@@ -186,7 +186,9 @@ class MixtralModel(nn.Module):
     @torch.no_grad()
     def decode_step(self, token: torch.Tensor, cache, pos: int, ep=None) -> torch.Tensor:
         """One new token per sequence at position ``pos``; returns its logits ``[B, vocab]``. On an 8-bit
-        cache ``token`` may be ``[B, S]``, S > 1 (a draft to check); the logits are then ``[B, S, vocab]``."""
+        cache ``token`` may be ``[B, S]``, S > 1 (a draft to check); the logits are then ``[B, S, vocab]``.
+        Where only the first are accepted, :meth:`rewind` takes the others back before the next step: left
+        there, they would keep the scale of the block they share with the tokens before them."""
         B = token.shape[0]
         S = check_draft(token, cache)
         x = self.embed(token.reshape(B * S)).contiguous()
@@ -196,6 +198,12 @@ class MixtralModel(nn.Module):
             x = layer(x, B, S, rope_p, self.impl, ep=ep, cache=c, pos=pos)
         logits = self._logits(x)
         return logits if S == 1 else logits.view(B, S, -1)
+
+    @torch.no_grad()
+    def rewind(self, cache, pos: int) -> None:
+        """Take back the tokens from position ``pos`` on of the last :meth:`decode_step`, a draft of 2 to 16
+        tokens of which only the first were accepted (:func:`flextensor_b200.models.kv_cache.rewind`)."""
+        rewind(cache, pos)
 
     @torch.no_grad()
     def generate(self, tokens: torch.Tensor, max_new: int, ep=None, cache_dtype=torch.bfloat16) -> torch.Tensor:

@@ -158,7 +158,10 @@ def kv_append_q8(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     afresh; one that holds earlier tokens of the sequence keeps the larger of its scale and the new
     tokens', and its codes are rounded again when that grows. A NaN or infinity makes its block's
     scale NaN, so that attention over it answers NaN. Codes outside the written tokens and their
-    blocks' earlier ones stay as they were. A sequence whose device-side ``pos`` / ``n_new`` do not
+    blocks' earlier ones stay as they were. So a block's codes depend on the order of its writes (rounded at
+    each growth of the scale, at most one step of the last scale off in all), and writing a position again
+    does not bring back the scale and codes from before its first writing: a caller that checks drafts
+    keeps the open block (``models.kv_cache.rewind`` does so for the decoder models). A sequence whose device-side ``pos`` / ``n_new`` do not
     fit the cache is left alone and recorded in ``native.device_error``."""
     if isinstance(pos, torch.Tensor):
         native.lib().kv_append_q8(k, v, k_cache, v_cache, k_scale, v_scale, pos, 0, n_new, block)

@@ -16,7 +16,7 @@ if not torch.cuda.is_available():  # pragma: no cover
 
 import flextensor_b200 as ft  # noqa: E402
 from flextensor_b200 import ops  # noqa: E402
-from flextensor_b200.models.kv_cache import QuantizedKV  # noqa: E402
+from flextensor_b200.models.kv_cache import QuantizedKV, new_layer_cache, rewind, store  # noqa: E402
 from flextensor_b200.models.llama import LlamaModel, init_llama_params_, tiny_llama  # noqa: E402
 from flextensor_b200.models.mixtral import MixtralModel, MixtralStack, init_mixtral_params_, tiny_mixtral  # noqa: E402
 from flextensor_b200.ops import native  # noqa: E402
@@ -181,4 +181,76 @@ def test_layers_with_and_without_the_few_token_path(kw, ids):
     cfg.moe_decode = False
     b = m(x.clone(), 1, 9, rope)
     assert near(a, b, 2 ** -7)  # one rounding of each path's output, and of the loop's h
+    assert native.device_error(reset=True) == 0
+
+
+def same_until(a, b, pos, block=64):
+    """The codes and scales of the tokens before ``pos``, bit for bit."""
+    blocks = -(-pos // block)
+    return all(torch.equal(x[:, :pos].view(torch.int8), y[:, :pos].view(torch.int8)) for x, y in zip(a[:2], b[:2])) and \
+        all(torch.equal(x[:, :blocks], y[:, :blocks]) for x, y in zip(a[2:4], b[2:4]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pos,n", [(70, 4), (64, 3), (1, 16), (62, 6)])
+@pytest.mark.parametrize("size", [100.0, float("nan")])
+def test_rejected_tokens_leave_no_trace(dtype, pos, n, size):
+    """Rejected tokens far larger than those before, or NaN: codes and scales as without them."""
+    g = torch.Generator(device=DEV).manual_seed(9)
+    old, new, one = ([torch.randn(2, s, 3, 128, device=DEV, generator=g).bfloat16() for _ in range(2)] for s in (pos, n, 1))
+    for accepted in (0, 1, n):
+        cache, want = (new_layer_cache(2, pos + n + 1, 3, 128, DEV, dtype) for _ in range(2))
+        k, v = (x.clone() for x in new)
+        for x in (k, v):
+            x[:, accepted:] *= size
+        for c in (cache, want):
+            store(c, *old, 0)
+        store(cache, k, v, pos)
+        if accepted:
+            store(want, k[:, :accepted], v[:, :accepted], pos)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            rewind([cache], pos + accepted)
+        torch.cuda.current_stream().wait_stream(side)
+        assert same_until(cache, want, pos + accepted)
+        for c in (cache, want):
+            store(c, *one, pos + accepted)
+        assert same_until(cache, want, pos + accepted + 1)
+    assert native.device_error(reset=True) == 0
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("family", ["llama", "mixtral"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_rejected_draft_costs_nothing(family, dtype):
+    """A draft of large keys and values (its pass runs with larger norm weights), rejected: the steps after it
+    are bit for bit those of a run without it, and nothing like them where it is left in the cache."""
+    m = build(family)
+    g = torch.Generator(device=DEV).manual_seed(10)
+    S, n = 70, 4
+    tokens = torch.randint(0, m.cfg.vocab, (3, S + n + 2), device=DEV, generator=g)
+    norms = [(layer if family == "llama" else layer.attn).attn_norm for layer in m.layers]
+
+    def run(draft, back):
+        cache = m.new_cache(3, S + n + 2, dtype=dtype)
+        m.prefill(tokens[:, :S], cache)
+        if draft:
+            for w in norms:
+                w *= 64
+            m.decode_step(tokens[:, S:S + n], cache, S)
+            for w in norms:
+                w /= 64
+        if back:
+            m.rewind(cache, S)
+        return [m.decode_step(tokens[:, S + n + i], cache, S + i) for i in range(2)], cache
+
+    want, clean = run(False, False)
+    got, cache = run(True, True)
+    assert all(same_until(a, b, S + 2) for a, b in zip(cache, clean))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    left, cache = run(True, False)
+    assert not same_until(cache[0], clean[0], S)
+    plain = m.new_cache(3, S + n + 2)
+    m.rewind(plain, 5)  # bf16: nothing to do
     assert native.device_error(reset=True) == 0
