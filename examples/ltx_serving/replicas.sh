@@ -39,5 +39,11 @@ for ((r = 0; r < REPLICAS; r++)); do
   pids+=($!)
 done
 trap 'kill "${pids[@]}" 2>/dev/null || true' EXIT INT TERM
-sleep 1  # an nginx that ends at once (its port taken) ends the replicas: let them start, so that each has said so
-nginx -c "$HERE/nginx.conf" -g "daemon off;"
+rc=0
+nginx -c "$HERE/nginx.conf" -g "daemon off;" || rc=$?
+# nginx ended by itself (at once where its port is taken): the replicas have 5 s to end by themselves, too
+for ((i = 0; i < 50; i++)); do
+  [ -n "$(jobs -rp)" ] || break
+  sleep 0.1
+done
+exit "$rc"

@@ -89,3 +89,49 @@ def test_profile_dir_is_required(tmp_path):
     e = {k: v for k, v in os.environ.items() if k != "PROFILE_DIR"}
     r = subprocess.run(["bash", SCRIPT], env=e, capture_output=True, text=True, timeout=30)
     assert r.returncode != 0 and "PROFILE_DIR" in r.stderr
+
+
+def _run_with(tmp_path, stubs, **env):
+    """The launcher with stubs of their own text for python, nginx and sleep: (result, log lines)."""
+    if shutil.which("bash") is None:
+        pytest.skip("bash not available")
+    bindir = tmp_path / "bin"
+    bindir.mkdir()
+    for name, text in stubs.items():
+        p = bindir / name
+        p.write_text("#!/usr/bin/env bash\n" + text)
+        p.chmod(p.stat().st_mode | stat.S_IXUSR)
+    log = tmp_path / "calls.log"
+    log.write_text("")
+    e = dict(os.environ, PATH=f"{bindir}:{os.environ['PATH']}", STUB_LOG=str(log), REAL_SLEEP=shutil.which("sleep"),
+             PROFILE_DIR="/tmp/prof", REPLICAS="3", **env)
+    r = subprocess.run(["bash", SCRIPT], env=e, capture_output=True, text=True, timeout=60)
+    return r, log.read_text().split("\n")
+
+
+def test_nginx_starts_without_delay(tmp_path):
+    """Nothing sleeps between the replicas' start and nginx."""
+    r, lines = _run_with(tmp_path, {"python": "exit 0", "nginx": 'echo nginx >> "$STUB_LOG"',
+                                    "sleep": 'echo sleep >> "$STUB_LOG"\nexec "$REAL_SLEEP" "$@"'})
+    assert r.returncode == 0 and lines[0] == "nginx"
+
+
+@pytest.mark.parametrize("rc", [0, 3])
+def test_an_nginx_that_ends_lets_replicas_finish(tmp_path, rc):
+    """Replicas that end by themselves two seconds later are not cut off; nginx's status is the launcher's."""
+    r, lines = _run_with(tmp_path, {"python": '"$REAL_SLEEP" 2\necho replica >> "$STUB_LOG"', "nginx": f"exit {rc}"})
+    assert r.returncode == rc and lines.count("replica") == 3
+
+
+def test_an_nginx_that_ends_ends_the_replicas(tmp_path):
+    """Replicas that go on are ended."""
+    r, lines = _run_with(tmp_path, {"python": 'trap \'echo ended >> "$STUB_LOG"; kill $!; exit 0\' TERM\n"$REAL_SLEEP" 40 &\nwait',
+                                    "nginx": "exit 0"})
+    assert r.returncode == 0
+    import time
+    for _ in range(50):
+        lines = (tmp_path / "calls.log").read_text().split("\n")
+        if lines.count("ended") == 3:
+            break
+        time.sleep(0.1)
+    assert lines.count("ended") == 3
