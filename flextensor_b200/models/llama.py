@@ -147,9 +147,10 @@ class LlamaLayer(nn.Module):
 
     # ---------------------------------------------------------------- tensor parallel (one rank's shard)
     def forward_tp(self, x_local, B, S, rope, tp, cache=None, pos: int = 0):
-        """One rank's shard. ``cache`` = this rank's (k_cache, v_cache) ``[B, L_max, hk, 128]``:
-        prefill (``pos == 0``) stores positions [0, S); a decode step (S == 1) appends position
-        ``pos`` and attends over [0, pos] with the split-KV decode kernel."""
+        """One rank's shard. ``cache`` = this rank's (k_cache, v_cache) ``[B, L_max, hk, 128]`` or its
+        8-bit :class:`~flextensor_b200.models.kv_cache.QuantizedKV`: prefill (``pos == 0``) stores positions
+        [0, S); a decode step (S == 1, or several tokens on an 8-bit cache) appends from position ``pos`` on
+        and attends over all before and among them."""
         from flextensor_b200 import ops
 
         cfg, D = self.cfg, self.cfg.head_dim
@@ -386,7 +387,8 @@ class LlamaTP(nn.Module):
     def forward(self, x_local: torch.Tensor, B: int, S: int, rope, cache=None, pos: int = 0) -> torch.Tensor:
         """x_local ``[B*S/world, dim]`` (this rank's token rows) -> same rows after all layers.
         Each layer is called as a module (``layers.*`` are offload units). ``cache``: from
-        :meth:`new_cache` (prefill at ``pos == 0``, then one decode step per call with S == 1)."""
+        :meth:`new_cache` (prefill at ``pos == 0``, then one decode step per call with S == 1; on an 8-bit
+        cache S > 1 is a draft, which ``models.kv_cache.rewind`` takes back)."""
         single = self.world == 1  # one rank: plain native layers, no collectives
         for i, L in enumerate(self.layers):
             x_local = L(x_local, B, S, rope, tp=None if single else self, cache=None if cache is None else cache[i],
