@@ -112,3 +112,14 @@ def test_runs(seed):
             assert got.get((b, hg), {}) == {u: 1 for u in range(units)}
             if units:
                 assert merged(lens, hgs, ut, sms, b, hg) == sorted(partials[b, hg])
+
+
+def test_constants_are_the_kernel_s():
+    import os
+    import re
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = open(os.path.join(root, "flextensor_b200", "ops", "csrc", "cache_q8_sm100.cu")).read()
+    value = lambda name: int(re.search(rf"constexpr int {name} = (\d+);", text).group(1))  # noqa: E731
+    assert (value("WARPS"), value("ENTRY"), value("UNIT")) == (WARPS, ENTRY, 32)
+    assert re.search(r"units_of_tile\(int column_tiles\) \{ return column_tiles == 1 \? 2 : 1; \}", text)  # ut of test_runs

@@ -169,3 +169,17 @@ def test_one_tensor_map_for_all_experts(distances, one):
     for d in distances:
         w.append(w[-1] + d)
     assert native.lib().moe_decode_one_map(w) == one
+
+
+def test_model_constants_are_the_kernel_s():
+    import os
+    import re
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = open(os.path.join(root, "flextensor_b200", "ops", "csrc", "moe_decode_sm100.cu")).read()
+    value = lambda name: int(re.search(rf"constexpr int {name} = (\d+);", text).group(1))  # noqa: E731
+    assert (value("BM"), value("BK"), value("MIN_CHUNKS")) == (128, 64, 4)
+    head = open(os.path.join(root, "flextensor_b200", "ops", "csrc", "ft_moe_decode.h")).read()
+    limit = lambda name: int(re.search(rf"constexpr int {name} = (\d+);", head).group(1))  # noqa: E731
+    assert (ops.MOE_DECODE_MAX_TOKENS, ops.MOE_DECODE_MAX_EXPERTS, ops.MOE_DECODE_MAX_TOPK) == \
+        (limit("kMoeDecMaxTokens"), limit("kMoeDecMaxExperts"), limit("kMoeDecMaxTopk"))
