@@ -62,23 +62,6 @@ constexpr int HD = 128;  // head dim
 // Every kernel here is launched so that it may start while the kernel before it in the stream ends
 // (programmatic serialization): it waits for that kernel's results before it reads any memory. No load
 // takes the non-coherent path, which that wait says nothing about.
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-template <class... P, class... A>
-cudaError_t launch_overlapped(void (*kernel)(P...), unsigned grid, int threads, int smem, cudaStream_t stream, const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = stream;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
-}
 
 // ------------------------------------------------------------------------------------ writing
 struct AppendArgs {
@@ -231,7 +214,7 @@ cudaError_t launch_append(AppendArgs a, int format, cudaStream_t stream) {
   const long long grid = (long long)a.B * 2 * a.n_rel * a.Hk;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
   return launch_overlapped(format == CACHE_INT8 ? cache_append_kernel<BLOCK, CACHE_INT8> : cache_append_kernel<BLOCK, CACHE_E4M3>,
-                           (unsigned)grid, 32 * Shape::WARPS, 0, stream, a);
+                           dim3((unsigned)grid), 32 * Shape::WARPS, 0, stream, a);
 }
 
 // ------------------------------------------------------------------------------------ attention
@@ -669,20 +652,6 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_
       : "memory");
 }
 
-// A wait that runs out (2 s) is recorded and answered with false.
-__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t phase) {
-  const uint32_t a = smem_u32(bar);
-  if (mbar_try_wait(a, phase)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait(a, phase)) {
-    if ((unsigned long long)(clock64() - t0) > FT_WAIT_LIMIT_CYCLES) {
-      record_error(kErrWaitTimeout);
-      return false;
-    }
-  }
-  return true;
-}
-
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
@@ -1010,7 +979,7 @@ cudaError_t launch_decode(const CUtensorMap& tk, const CUtensorMap& tv, const De
     if (err == cudaSuccess && dev < 64) ready[dev] = true;
   }
   if (err != cudaSuccess) return err;
-  return launch_overlapped(cache_decode_kernel<NT, FMT>, (unsigned)sms, 32 * WARPS, smem, stream, tk, tv, a);
+  return launch_overlapped(cache_decode_kernel<NT, FMT>, dim3((unsigned)sms), 32 * WARPS, smem, stream, tk, tv, a);
 }
 
 template <int NT>
@@ -1018,7 +987,7 @@ cudaError_t launch_merge(const DecArgs& a, cudaStream_t stream) {
   // CTAs of four warps, or of one row's where that is more: small ones fill the SMs evenly
   const int warps = std::max(4, a.merge_per_row), rows_here = warps / a.merge_per_row;
   const int rows = a.B * a.Hk * a.R;
-  return launch_overlapped(cache_merge_kernel<NT>, (unsigned)((rows + rows_here - 1) / rows_here), 32 * warps, 0, stream, a);
+  return launch_overlapped(cache_merge_kernel<NT>, dim3((unsigned)((rows + rows_here - 1) / rows_here)), 32 * warps, 0, stream, a);
 }
 
 }  // namespace

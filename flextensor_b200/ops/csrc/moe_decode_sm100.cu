@@ -79,22 +79,6 @@ struct Maps {
 };
 
 __device__ __forceinline__ void fence_proxy_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-// A wait that runs out (2 s) is recorded; the caller then skips its work but keeps its barriers.
-__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t phase) {
-  const uint32_t a = smem_u32(bar);
-  if (mbar_try_wait(a, phase)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try_wait(a, phase)) {
-    if ((unsigned long long)(clock64() - t0) > FT_WAIT_LIMIT_CYCLES) {
-      record_error(kErrWaitTimeout);
-      return false;
-    }
-  }
-  return true;
-}
 
 // ------------------------------------------------------------------------------------ routing
 constexpr int LOGIT_WARPS = 8;
@@ -720,21 +704,6 @@ bool weight_maps(Maps<N>& m, const __nv_bfloat16* const* w, int E, int inner, in
       if (!make_tmap_3d_bf16(&m.w[e], w[e], inner, rows, 1, ld, 0, BK, BM)) return false;
     return true;
   }
-}
-
-template <class... P, class... A>
-cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = stream;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <bool UP, int N>

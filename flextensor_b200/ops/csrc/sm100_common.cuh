@@ -129,6 +129,42 @@ __device__ __forceinline__ bool mbar_test_wait(uint32_t bar_addr, uint32_t phase
   return ok != 0;
 }
 
+// A wait that runs out (2 s) is recorded and answered with false. Unlike mbar_wait_t it looks at its own
+// clock only, not at the error word: an error that another kernel recorded earlier does not end it.
+__device__ __forceinline__ bool bounded_wait(uint64_t* bar, uint32_t phase) {
+  const uint32_t a = smem_u32(bar);
+  if (mbar_try_wait(a, phase)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(a, phase)) {
+    if ((unsigned long long)(clock64() - t0) > FT_WAIT_LIMIT_CYCLES) {
+      record_error(kErrWaitTimeout);
+      return false;
+    }
+  }
+  return true;
+}
+
+// ------------------------------------------------------------------ programmatic launches
+// A kernel launched with launch_overlapped may start while the kernel before it in the stream ends; it
+// waits for that kernel's results with pdl_wait, and lets the next one start with pdl_launch.
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... P, class... A>
+cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = stream;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 enum MbarWaitMode : int { kWaitProbe = 0, kWaitSleep = 1, kWaitSpin = 2 };
 
 // Bounded wait for the barrier phase with parity `phase` to complete. kWaitProbe: try_wait
