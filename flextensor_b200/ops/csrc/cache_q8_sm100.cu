@@ -386,11 +386,11 @@ struct RowState {
 
 // The scales of a tile's 16-key groups, keys' and values'.
 // In the reference a value scale counts as at least 2^-60, so a key's p is at most 2^75 (blocks of zeros), and
-// as finite, so that an infinite one stays with the rows that see it.
-// Tiles with a scale outside 2^+-30 compute p and p * vs each by itself, the others p as (p * vs) / vs, which
-// has fp32's precision beside value scales up to 2^90 times larger. Values of scales below 2^-84 underflow to 0.
+// as finite, so that an infinite one stays with the rows that see it. Tiles with a scale outside 2^+-30 compute
+// p by itself, the others as (p * vs) / vs, which has fp32's precision beside value scales up to 2^90 times
+// larger. Values of scales below 2^-84 underflow to 0.
 constexpr float V_SCALE_MIN = 0x1p-60f, V_SCALE_MAX = 0x1.fffffep127f, V_SCALE_ODD = 0x1p30f;
-// The sums of p are kept 2^20 times larger: at most 2^127 over 2^32 keys. The key that weighs most adds
+// p and its sums are kept 2^20 times larger: at most 2^127 over 2^32 keys. The key that weighs most has
 // 2^(27 - 122) or more beside bf16's largest values (whose scale is 2^122 in int8), and one 2^31 times lighter
 // is still a normal number; beside the largest scale that fp32 holds, one 2^25 times lighter.
 constexpr float SUM_LOG2 = 20.f, SUM_UNIT = 0x1p20f;
@@ -508,13 +508,13 @@ __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT
     } else {  // p * vs is 0 for a scale of 0, NaN for NaN, and 0 for what the column does not see
 #pragma unroll
       for (int mt = 0; mt < MT; mt++) {
-        const float lw = lg2f(sc.v[mt]);
+        const float v = sc.v[mt] * (1.f / SUM_UNIT);
         float w[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float x = s[mt][nt][e] - ref[e & 1];
-          st.l[nt][e & 1] += ex2f(x + SUM_LOG2);
-          w[e] = masked && mt * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1] ? 0.f : ex2f(x + lw);
+          const float p = ex2f(s[mt][nt][e] + (SUM_LOG2 - ref[e & 1]));
+          st.l[nt][e & 1] += p;
+          w[e] = masked && mt * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1] ? 0.f : p * v;
         }
         weights(mt, w[0], w[1], w[2], w[3]);
       }
