@@ -507,10 +507,14 @@ std::pair<Tensor, int> decode_attention_q8(const Tensor& q, const Tensor& kc, co
   for (int64_t first = 0; first < Sq; first += step) {
     p.Sq = (int)std::min<int64_t>(step, Sq - first);
     p.later = (int)(Sq - first - p.Sq);
+    if (!each) {  // a known length ends with these queries
+      p.len_all = p.max_len = (int)std::max<int64_t>(0, len_all - p.later);
+      p.later = 0;
+    }
     p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr()) + first * p.q_tok;
     p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr()) + first * p.o_tok;
     check_ok(ft::cache_decode(p, at::cuda::getCurrentCUDAStream()), op);
-    launches += p.max_len > p.later ? 2 : 1;
+    launches += p.max_len > 0 ? 2 : 1;
   }
   return {o, launches};
 }

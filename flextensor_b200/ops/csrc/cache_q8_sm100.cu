@@ -230,7 +230,8 @@ constexpr int ENTRY = 2;
 constexpr int MERGE_WARPS = 16;  // at most
 
 struct DecArgs {
-  int B, Sq, Hq, Hk, L, G, R, n_group;  // R = Sq * G query rows of a KV head in n_group groups of 8 * NT
+  int B, Hq, Hk, L, G, R, n_group;      // R query rows of a KV head (queries x G) in n_group groups of 8 * NT
+  int to_end;                           // tokens of a sequence from the first query's to its last
   int block_shift;
   int heads, keys;                      // (head, group) units and key tiles side by side in a CTA: heads * keys = WARPS
   int per;                              // Hk * n_group / heads: steps of heads in a sequence
@@ -242,7 +243,7 @@ struct DecArgs {
   CacheSide k, v;
   int one_b[2], one_h[2];               // keys / values: the cache is broadcast over sequences / heads (stride 0)
   const int* kv_len;
-  int len_all, max_len, later;          // later: tokens of each sequence behind the last query's
+  int len_all, max_len;
   float scale_log2;                     // softmax scale * log2(e)
   float* part_o;                        // [steps of heads + runs][WARPS][8 * NT][128]
   float2* part_ml;                      // [steps of heads + runs][WARPS][8 * NT] reference and sum
@@ -544,7 +545,7 @@ __device__ __forceinline__ void attend_tile(RowState<NT>& st, const QueryFrag<NT
 }
 
 __device__ __forceinline__ int seq_len(const DecArgs& a, int b) {
-  return max(0, min(a.kv_len ? a.kv_len[b] : a.len_all, a.max_len) - a.later);
+  return max(0, min(a.kv_len ? a.kv_len[b] : a.len_all, a.max_len));
 }
 __device__ __forceinline__ int seq_units(const DecArgs& a, int b) { return (seq_len(a, b) + UNIT - 1) / UNIT; }
 
@@ -750,7 +751,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
       for (int i = 0; i < 2; i++) {
         st.m[nt][i] = -INFINITY;
         st.l[nt][i] = 0.f;
-        sees[nt][i] = len - a.Sq + 1 + min(qf.row[nt][i], a.R - 1) / a.G;
+        sees[nt][i] = len - a.to_end + 1 + min(qf.row[nt][i], a.R - 1) / a.G;
 #pragma unroll
         for (int j = 0; j < 8; j++) st.o[j][nt][i] = st.o[j][nt][2 + i] = 0.f;
       }
@@ -784,7 +785,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
         lim[nt][0] = min(sees[nt][0] - key0, here);
         lim[nt][1] = min(sees[nt][1] - key0, here);
       }
-      const bool masked = here < 16 * MT || key0 + 16 * MT > len - a.Sq + 1;
+      const bool masked = here < 16 * MT || key0 + 16 * MT > len - a.to_end + 1;
       const int valid = min(len - key0, here);
       const uint32_t kb = smem_u32(sm.slot[warp][sk]), vb = smem_u32(sm.slot[warp][s]);
       auto kt = [&](int r, int piece) { return lds128(kb + r * 128 + ((piece ^ (r & 7)) << 4)); };
@@ -941,7 +942,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) cache_merge_kernel(const __g
   const float inv = 1.f / L;
   uint2 out = make_uint2(pack_bf16x2(acc.x * SUM_UNIT * inv, acc.y * SUM_UNIT * inv),
                          pack_bf16x2(acc.z * SUM_UNIT * inv, acc.w * SUM_UNIT * inv));
-  if (len - a.Sq + 1 + r / a.G <= 0) out = make_uint2(0, 0);  // the row sees no key
+  if (len - a.to_end + 1 + r / a.G <= 0) out = make_uint2(0, 0);  // the row sees no key
   *reinterpret_cast<uint2*>(a.o + b * a.o_b + (long long)(r / a.G) * a.o_tok + (long long)(h * a.G + r % a.G) * a.o_h + 4 * lane) = out;
 }
 
@@ -1028,7 +1029,7 @@ cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream) {
   if (p.Hk <= 0 || p.Hq % p.Hk) return cudaErrorInvalidValue;
   DecArgs a;
   a.B = p.B;
-  a.Sq = p.Sq;
+  a.to_end = p.Sq + p.later;
   a.Hq = p.Hq;
   a.Hk = p.Hk;
   a.L = p.L;
@@ -1049,7 +1050,6 @@ cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream) {
   a.kv_len = p.kv_len;
   a.len_all = p.len_all;
   a.max_len = p.max_len;
-  a.later = p.later;
   a.scale_log2 = p.scale * 1.4426950408889634f;
   a.heads = heads_of(p);
   a.keys = WARPS / a.heads;
@@ -1065,7 +1065,7 @@ cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream) {
   const long long expect = (a.runs / head_steps_of(p) + 1) * a.keys;
   a.merge_per_row = expect >= 64 ? 16 : expect >= 32 ? 8 : expect >= 16 ? 4 : expect >= 8 ? 2 : 1;
   const bool one = col_tiles(p) == 1;
-  if (p.max_len > p.later) {  // without keys there may be no memory to map; the merge alone writes the zeros
+  if (p.max_len > 0) {  // without keys there may be no memory to map; the merge alone writes the zeros
     CUtensorMap tk, tv;
     if (!side_map(&tk, p.side[0], p, a.one_b[0], a.one_h[0]) || !side_map(&tv, p.side[1], p, a.one_b[1], a.one_h[1]))
       return cudaErrorInvalidValue;

@@ -44,7 +44,7 @@ struct CacheDecodeProblem {
   float* scratch = nullptr;                // cache_decode_scratch_floats(p) floats
 };
 size_t cache_decode_scratch_floats(const CacheDecodeProblem& p);
-// two kernels; where no key may count (max_len <= later), the second alone
+// two kernels; where no key may count (max_len 0), the second alone
 cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream);
 int cache_device_error(bool reset);
 
