@@ -175,8 +175,8 @@ def decode_attention_q8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
                         max_len: int | None = None, scale: float | None = None,
                         out: torch.Tensor | None = None) -> torch.Tensor:
     """:func:`decode_attention` over a cache written by :func:`kv_append_q8` (or any codes with
-    scales that are not negative; e4m3 codes must be finite; value scales below 2**-84 count as 0, and
-    a sequence's others should lie within 2**90 of one another).
+    scales that are not negative; e4m3 codes must be finite; value scales below 2**-84 count as 0, others
+    may be as large as fp32 holds, but a sequence's should lie within 2**90 of one another).
 
     ``q [B, Hq, 128]``, or ``[B, Sq, Hq, 128]`` for the last Sq tokens of each sequence, whose keys
     are in the cache already: query i sees keys ``[0, kv_len - Sq + 1 + i)``; one that sees none gets
@@ -205,7 +205,8 @@ def moe_decode(x: torch.Tensor, router: torch.Tensor, w_gate_up, w_down, topk: i
     ``x [T, D]``, ``router [E, D]`` (at most 128 experts); ``w_gate_up`` / ``w_down``: a sequence of one
     ``[2F, D]`` (gate and up rows interleaved) / ``[D, F]`` tensor per expert, or one stacked tensor.
     Each token takes the ``topk`` (at most 8) experts of the largest router logits (fp32; equal ones
-    go to the lower index) weighted by the softmax over those. ``out`` may be ``residual`` or ``x``."""
+    go to the lower index) weighted by the softmax over those. ``out`` may be ``residual`` or ``x``, but may
+    not overlap them otherwise."""
     if isinstance(w_gate_up, torch.Tensor):
         w_gate_up = w_gate_up.unbind(0)
     if isinstance(w_down, torch.Tensor):

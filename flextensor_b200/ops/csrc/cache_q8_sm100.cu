@@ -2,9 +2,10 @@
 // and decode attention over it, head_dim 128, for sm_100a.
 //
 // Writing. A block's scale is the smallest power of two s with max|x| <= qmax * s (qmax 127 for
-// int8, 448 for e4m3), so x / s is exact and a code depends on the value alone; a block that
-// already holds tokens keeps the larger of its old scale and the new tokens', and its old codes
-// are rounded again when the scale grew. The largest magnitude is found on the bf16 bit patterns
+// int8, 448 for e4m3), so x / s is exact and a block written at once has codes that depend on its
+// values alone. A block that already holds tokens keeps the larger of its old scale and the new
+// tokens', and its old codes are rounded again when the scale grew: written in several calls, its
+// codes depend on their order too (by at most one step of the last scale). The largest magnitude is found on the bf16 bit patterns
 // (sign cleared, as 16-bit integers): NaN and infinity compare above every finite value, and a
 // block that received one gets the scale NaN, which reaches every output that reads the block.
 //
@@ -36,8 +37,9 @@
 // Scales: a score is (q . codes) * ks, and the weight of a value's codes is p * vs. The running
 // reference is 7 below the maximum of score + log2(vs) (in log2 units), so that p * vs is at most 2^15
 // whatever the scales are and f16 holds it to 2^-11, or to 2^-32 of the largest weight where that is
-// more (a million keys that weigh less together still add up to 2^-12); the sum l takes p in fp32. q is scaled by a power
-// of two per row into f16 (exact but for elements below 2^-24 of the row's largest).
+// more (a million keys that weigh less together still add up to 2^-12); the sum l takes p in fp32. q is
+// scaled by a power of two per row into f16, the row's largest element to 1 .. 2: elements below 2^-17 of it
+// lose bits there, by at most 2^-25 of the largest (f16's numbers are 2^-24 apart below 2^-14).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -117,9 +119,9 @@ __device__ __forceinline__ uint32_t recode4(uint32_t w, float ratio) {
 // A block belongs to BLOCK / 16 warps, whose lanes hold its new tokens in registers (eight 16-byte pieces
 // each) between the maximum and the rounding, so they are read once; a CTA of at least four warps takes
 // consecutive blocks of one sequence and KV head, keys or values. Bound by HBM for prompts (32 x 2048
-// tokens, 8 heads: 403 MB in 61-63 us at blocks of 16 to 64 tokens, the rate of a copy; 66 at 128, 94 at
-// 256, where few large CTAs overlap their loads and stores badly) and by the launch for single tokens
-// (3.0 us on the device).
+// tokens, 8 heads: 403 MB in 60-61 us at blocks of 16 to 64 tokens, the rate of a copy; 66 at 128, 94 at
+// 256: 512 threads of 80 and more registers leave room for one CTA an SM, whose loads, barrier and stores
+// then overlap with no other's) and by the launch for single tokens (3.0 us on the device).
 template <int BLOCK>
 struct AppendShape {
   static constexpr int WARPS_PER_BLOCK = BLOCK / 16, WARPS = WARPS_PER_BLOCK > 4 ? WARPS_PER_BLOCK : 4;
@@ -665,8 +667,8 @@ struct DecSmem {
   uint64_t full[WARPS][SLOTS];
 };
 
-// Bound by HBM where sequences are long (131071 tokens, 8 heads, e4m3: 268 MB in 53 us with the merge,
-// 5.1 TB/s; 32 x 2304 tokens, int8: 152 MB in 35 us, of which 24 us stream) and by latency where they
+// Bound by HBM where sequences are long (131071 tokens, 8 heads, e4m3: 268 MB in 51-53 us with the merge,
+// 5.1-5.3 TB/s; 32 x 2304 tokens, int8: 152 MB in 35 us, of which 24 us stream) and by latency where they
 // are short. The loads of a head's queries and scales come before the copies, which would hold them
 // up for 5 us in the memory's queues.
 template <int NT, int FMT>
