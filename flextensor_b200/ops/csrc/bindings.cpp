@@ -496,17 +496,17 @@ std::pair<Tensor, int> decode_attention_q8(const Tensor& q, const Tensor& kc, co
   p.scale = (float)scale;
   p.num_sms = num_sms_for(kc.get_device());
   if (q.numel() == 0) return {o, 0};
-  while (p.Sq > 1 && ft::cache_decode_scratch_floats(p) * sizeof(float) > kCacheDecodeScratchBytes) p.Sq = (p.Sq + 1) / 2;
-  const int step = p.Sq;
-  if (step < Sq && shares_memory(o, q))  // a launch's outputs are written before the next one's queries are read
+  const ft::CacheDecodePlan plan = ft::cache_decode_plan(p, kCacheDecodeScratchBytes);
+  if (plan.queries.size() > 1 && shares_memory(o, q))  // a launch's outputs are written before the next one's queries are read
     TORCH_CHECK(q.const_data_ptr() == o.const_data_ptr() && lattice(q) == lattice(o), op,
                 ": out may be q, but must not overlap it otherwise");
-  const auto scratch = c10::cuda::CUDACachingAllocator::get()->allocate(ft::cache_decode_scratch_floats(p) * sizeof(float));
+  const auto scratch = c10::cuda::CUDACachingAllocator::get()->allocate(plan.scratch_bytes);
   p.scratch = static_cast<float*>(scratch.get());
   int launches = 0;
-  for (int64_t first = 0; first < Sq; first += step) {
-    p.Sq = (int)std::min<int64_t>(step, Sq - first);
-    p.later = (int)(Sq - first - p.Sq);
+  int64_t first = 0;
+  for (const int queries : plan.queries) {
+    p.Sq = queries;
+    p.later = (int)(Sq - first - queries);
     if (!each) {  // a known length ends with these queries
       p.len_all = p.max_len = (int)std::max<int64_t>(0, len_all - p.later);
       p.later = 0;
@@ -515,6 +515,7 @@ std::pair<Tensor, int> decode_attention_q8(const Tensor& q, const Tensor& kc, co
     p.o = reinterpret_cast<__nv_bfloat16*>(o.data_ptr()) + first * p.o_tok;
     check_ok(ft::cache_decode(p, at::cuda::getCurrentCUDAStream()), op);
     launches += p.max_len > 0 ? 2 : 1;
+    first += queries;
   }
   return {o, launches};
 }
@@ -1074,6 +1075,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_attention_q8", &decode_attention_q8, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("k_scale"), py::arg("v_scale"), py::arg("out"), py::arg("kv_len"), py::arg("len_all"),
         py::arg("max_len"), py::arg("block"), py::arg("scale"));
+  m.def("decode_attention_q8_plan", [](int B, int Sq, int Hq, int Hk, int num_sms) {
+    ft::CacheDecodeProblem p;
+    p.B = B;
+    p.Sq = Sq;
+    p.Hq = Hq;
+    p.Hk = Hk;
+    p.num_sms = num_sms;
+    const ft::CacheDecodePlan plan = ft::cache_decode_plan(p, kCacheDecodeScratchBytes);
+    return std::make_pair(plan.queries, plan.scratch_bytes);
+  });
   m.def("moe_decode", &moe_decode, py::arg("x"), py::arg("router"), py::arg("w_gate_up"), py::arg("w_down"),
         py::arg("topk"), py::arg("residual"), py::arg("out"));
   m.def("moe_decode_one_map", [](const std::vector<uint64_t>& w) {

@@ -997,6 +997,19 @@ cudaError_t launch_merge(const DecArgs& a, cudaStream_t stream) {
 
 size_t cache_decode_scratch_floats(const CacheDecodeProblem& p) { return (size_t)partials_of(p) * (HD + 2); }
 
+CacheDecodePlan cache_decode_plan(CacheDecodeProblem p, size_t most) {
+  CacheDecodePlan plan;
+  auto bytes = [&] { return cache_decode_scratch_floats(p) * sizeof(float); };
+  for (int rest = p.Sq, step = p.Sq; rest > 0; rest -= p.Sq) {
+    p.Sq = std::min(step, rest);
+    while (p.Sq > 1 && bytes() > most) p.Sq = (p.Sq + 1) / 2;
+    if (plan.queries.empty()) step = p.Sq;
+    plan.queries.push_back(p.Sq);
+    plan.scratch_bytes = std::max(plan.scratch_bytes, bytes());
+  }
+  return plan;
+}
+
 cudaError_t cache_append(const CacheAppendProblem& p, cudaStream_t stream) {
   if (p.B <= 0 || p.S <= 0 || p.Hk <= 0) return cudaSuccess;
   AppendArgs a;

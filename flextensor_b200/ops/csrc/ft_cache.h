@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <vector>
+
 namespace ft {
 
 enum CacheFormat : int { CACHE_INT8 = 0, CACHE_E4M3 = 1 };
@@ -44,6 +46,14 @@ struct CacheDecodeProblem {
   float* scratch = nullptr;                // cache_decode_scratch_floats(p) floats
 };
 size_t cache_decode_scratch_floats(const CacheDecodeProblem& p);
+// The p.Sq queries of a call in launches whose scratch stays within `most` bytes (where one query's does): their
+// numbers of queries, and the scratch that the largest takes. It does not grow with the queries alone: how many
+// heads stand side by side depends on what divides their number.
+struct CacheDecodePlan {
+  std::vector<int> queries;
+  size_t scratch_bytes = 0;
+};
+CacheDecodePlan cache_decode_plan(CacheDecodeProblem p, size_t most);
 // two kernels; where no key may count (max_len 0), the second alone
 cudaError_t cache_decode(const CacheDecodeProblem& p, cudaStream_t stream);
 int cache_device_error(bool reset);

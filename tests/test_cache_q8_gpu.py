@@ -533,3 +533,25 @@ def test_attention_of_many_queries_in_place():
     with pytest.raises(RuntimeError, match="overlap it otherwise"):
         ops.decode_attention_q8(q, *cache, L, block=block, out=shifted)
     assert torch.equal(ops.decode_attention_q8(q, *cache, L, block=block, out=q), want)
+
+
+def test_attention_of_many_queries_of_one_head():
+    """Launches of 502 queries (32 groups of rows, eight side by side) and a last one of 494 (31, one by one), whose
+    workspace is the larger."""
+    B, Sq, L, block = 64, 8024, 8100, 256
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    queries, _ = native.lib().decode_attention_q8_plan(B, Sq, 1, 1, sms)
+    assert len(set(queries)) > 1
+    cache = junk_cache("int8", 1, L, 1, block, 55)
+    shared = [c.expand(B, *c.shape[1:]) for c in cache]
+    q = bf16(56, 1, Sq, 1, 128, spread=False)
+    got = ops.decode_attention_q8(q.expand(B, Sq, 1, 128), *shared, L, block=block)
+    torch.cuda.synchronize()
+    assert native.device_error(reset=True) == 0
+    of = torch.arange(L, device=DEV) // block
+    k, v = (cache[i][0, :, 0].double() * cache[2 + i][0, of, 0].double()[:, None] for i in (0, 1))
+    for i in (0, 1, 501, 502, 4000, 7529, 7530, 7531, Sq - 1):
+        m = L - Sq + 1 + i
+        p = torch.softmax(k[:m] @ q[0, i, 0].double() * 128 ** -0.5, 0)
+        err = (got[:, i, 0].double() - p @ v[:m]).abs()
+        assert bool((err <= (p @ v[:m]).abs() * 2 ** -8 + (p @ v[:m].abs()) * 2 ** -9).all())

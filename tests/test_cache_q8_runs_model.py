@@ -123,3 +123,35 @@ def test_constants_are_the_kernel_s():
     value = lambda name: int(re.search(rf"constexpr int {name} = (\d+);", text).group(1))  # noqa: E731
     assert (value("WARPS"), value("ENTRY"), value("UNIT")) == (WARPS, ENTRY, 32)
     assert re.search(r"units_of_tile\(int column_tiles\) \{ return column_tiles == 1 \? 2 : 1; \}", text)  # ut of test_runs
+
+
+def scratch_bytes(B, Sq, Hq, Hk, sms):
+    """What one launch may write: a partial result (128 dims, reference, sum) for each row of every warp of
+    every piece, whose numbers stay below steps of heads + runs."""
+    rows = Sq * (Hq // Hk)
+    tiles = 2 if rows > 8 else 1
+    units = Hk * -(-rows // (8 * tiles))
+    return (B * units // side_by_side(units) + sms) * WARPS * 8 * tiles * 130 * 4
+
+
+def test_launches_of_many_queries_stay_within_the_workspace():
+    from flextensor_b200.ops import native
+
+    if not native.available():
+        pytest.skip("native extension not built")
+    rng = random.Random(7)
+    cases = [(64, 8024, 1, 1), (16, 1000, 64, 8), (32, 2048, 64, 8), (1, 1, 8, 1), (1, 100000, 7, 7), (256, 3, 96, 3)]
+    for _ in range(300):
+        Hk = rng.choice([1, 2, 3, 5, 7, 8])
+        cases.append((rng.choice([1, 3, 16, 64, 200]), int(2 ** rng.uniform(0, 14)), Hk * rng.choice([1, 2, 5, 6, 8, 16]), Hk))
+    split = 0
+    for B, Sq, Hq, Hk in cases:
+        for sms in (148, 132):
+            queries, held = native.lib().decode_attention_q8_plan(B, Sq, Hq, Hk, sms)
+            assert sum(queries) == Sq and min(queries) >= 1
+            assert held == max(scratch_bytes(B, n, Hq, Hk, sms) for n in queries)
+            assert held <= 256 << 20 or held == scratch_bytes(B, 1, Hq, Hk, sms)
+            if scratch_bytes(B, Sq, Hq, Hk, sms) <= 256 << 20:
+                assert queries == [Sq]
+            split += len(queries) > 1
+    assert split > 50
