@@ -16,7 +16,8 @@ if not torch.cuda.is_available():  # pragma: no cover
 
 import flextensor_b200 as ft  # noqa: E402
 from flextensor_b200 import ops  # noqa: E402
-from flextensor_b200.models.kv_cache import QuantizedKV, new_layer_cache, rewind, store  # noqa: E402
+from flextensor_b200.models.kv_cache import QuantizedKV  # noqa: E402
+from flextensor_b200.models.kv_cache import new_layer_cache, rewind, store  # noqa: E402
 from flextensor_b200.models.llama import LlamaModel, init_llama_params_, tiny_llama  # noqa: E402
 from flextensor_b200.models.mixtral import MixtralModel, MixtralStack, init_mixtral_params_, tiny_mixtral  # noqa: E402
 from flextensor_b200.ops import native  # noqa: E402
